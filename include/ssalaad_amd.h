@@ -647,6 +647,140 @@ int ssl_decode_rope_attention(const void* q, int64_t ldq, const void* k, int64_t
 int ssl_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, void* out,
                  int64_t ldo, int64_t rows, int64_t n, int32_t dtype, void* stream);
 
+/* -------------------------------------------------------------------------
+ * Serving from a paged key/value cache (no reference counterpart: its
+ * generation keeps no cache, ssalaad/inference/generate.py:1-26). Keys and
+ * values live in two pools of pages, [layers, pages, kv_heads, page, head_dim]
+ * with equal strides (elements; the features of one head contiguous, every
+ * stride and base 16-byte aligned). `table` [seqs, cols] int32 names the page
+ * of each run of `page` positions of a sequence, -1 where there is none.
+ * Every entry point takes one struct whose first member is its own size.
+ * Page numbers are checked on the device: a position whose table entry lies
+ * outside [0, pages) is neither read nor written.
+ * page: a power of two from 16 to 1024; head_dim 64, 128 or 256.
+ * ------------------------------------------------------------------------- */
+typedef struct {
+  int64_t bytes; /* of the enclosing argument struct */
+  void *k, *v;
+  int64_t layer_stride, page_stride, head_stride, slot_stride;
+  int64_t layers, pages, kv_heads, page, head_dim;
+  const int32_t* table;
+  int64_t table_stride, seqs, cols;
+  int64_t dtype;
+} ssl_paged_cache;
+
+/* ssl_paged_append — rotary embedding of new tokens' q and k, k and v written
+ * into the pages (one layer: the pools at layer 0):
+ *   x' = x · rsqrt(mean(x²) + eps) · norm        (where norm is given)
+ *   (a, b) -> (a·cos − b·sin, b·cos + a·sin)     a, b: the head's halves
+ * in fp32 with one rounding at the store. Token t belongs to sequence
+ * seq_ids[t] at positions[t]; cos/sin are fp32 [angles, head_dim / 2]. A
+ * position outside [0, angles) gives a zero row of q_out and, like one whose
+ * sequence or page is out of range, writes nothing into the pools. q_out is
+ * [tokens, heads, head_dim], contiguous; q, k, v have token and head strides. */
+typedef struct {
+  ssl_paged_cache cache;
+  const void* q;
+  int64_t q_token, q_head;
+  const void* k;
+  int64_t k_token, k_head;
+  const void* v;
+  int64_t v_token, v_head;
+  const float *cos, *sin;
+  int64_t cos_stride, sin_stride, angles;
+  const void *q_norm, *k_norm;
+  double eps;
+  const int32_t *seq_ids, *positions;
+  void* q_out;
+  int64_t tokens, heads;
+} ssl_paged_append_args;
+int ssl_paged_append(const ssl_paged_append_args* args, void* stream);
+
+/* ssl_paged_attention — out[t, h] = Σ_j softmax_j(q[t, h]·k_j · scale) v_j over
+ * the positions j of the token's sequence with j <= p (p its own position) and,
+ * with a window > 0, j > p − window or j < sinks. Query head h reads key/value
+ * head h / (heads / kv_heads). A token that sees nothing gives zeros. Scores,
+ * softmax and sums are fp32, rounded once at the store.
+ *   cu NULL   one token per sequence: t is the sequence, p = lengths[t] − 1
+ *   cu        [seqs + 1] int32, ascending from 0: tokens cu[s] … cu[s+1] − 1
+ *             belong to sequence s and are its last ones (lengths[s] counts
+ *             them); tokens from cu[seqs] on give zeros
+ * Lengths are cut at cols · page. max_tokens and max_length (bounds of a
+ * sequence's tokens and length) shape the grid only: outputs do not depend on
+ * them beyond rounding. `workspace` (ssl_paged_attention_workspace_size bytes
+ * for the same arguments, 16-byte aligned, no initial contents) holds the
+ * partial sums of contexts that are split; calls that share it are ordered. */
+typedef struct {
+  ssl_paged_cache cache;
+  const void* q;
+  int64_t q_token, q_head;
+  void* out;
+  const int32_t *lengths, *cu;
+  int64_t tokens, heads, window, sinks;
+  double scale;
+  int64_t max_tokens, max_length;
+  void* workspace;
+  int64_t workspace_bytes;
+} ssl_paged_attention_args;
+int64_t ssl_paged_attention_workspace_size(const ssl_paged_attention_args* args);
+int ssl_paged_attention(const ssl_paged_attention_args* args, void* stream);
+
+/* Pages of sequences: refs [pages] int32 counts the table entries that name a
+ * page, 0 for a free one. Each call reads the state it is given and writes the
+ * new one into *_out arrays (contiguous, not overlapping the inputs).
+ *
+ * ssl_pages_free  the sequences seq_ids[0..n) end: their rows become -1, their
+ *   lengths 0, their pages lose one reference an entry. A sequence named twice
+ *   ends once; one out of range is passed over.
+ * ssl_pages_fork  dst[i] goes on as src[i] does: it shares the whole pages
+ *   (their references grow) and, where the last page is partly filled, gets the
+ *   lowest free page with those positions copied in every layer. Forks are
+ *   served in order, all from the state before the call. ok[i] (one byte) is 0
+ *   and nothing changes where src or dst is out of range, dst is not empty
+ *   (length 0) or named before, a page of src is out of range, or no page is
+ *   free. `workspace`: ssl_pages_fork_workspace_size(n) bytes.
+ * ssl_pages_compact  the pages in use (refs > 0) move to the lowest numbers:
+ *   with L of them, the i-th used page at or above L moves into the i-th free
+ *   one below it, in every layer; entries follow; live_out is L (int32).
+ *   `workspace`: ssl_pages_compact_workspace_size(pages) bytes. */
+typedef struct {
+  ssl_paged_cache cache;
+  const int32_t *lengths, *refs;
+  const int32_t *src, *dst; /* free: the sequences in dst */
+  int64_t n;
+  int32_t *table_out, *lengths_out, *refs_out;
+  uint8_t* ok;
+  int32_t* live_out;
+  void* workspace;
+  int64_t workspace_bytes;
+} ssl_pages_args;
+int ssl_pages_free(const ssl_pages_args* args, void* stream);
+int64_t ssl_pages_fork_workspace_size(int64_t n);
+int ssl_pages_fork(const ssl_pages_args* args, void* stream);
+int64_t ssl_pages_compact_workspace_size(int64_t pages);
+int ssl_pages_compact(const ssl_pages_args* args, void* stream);
+
+/* ssl_token_logprobs — for each row of logits [rows, ld] (vocab used):
+ *   logprob  = x[token] − log Σ exp(x)             (fp32; token int64)
+ *   entropy  = −Σ p log p
+ *   top_ids, top_logprobs [rows, top]: the top most likely tokens, descending,
+ *   equal logits in ascending order.
+ * The exponentials are fp32, their sums 64-bit. A token outside [0, vocab) has
+ * logprob NaN; a row with a NaN, a +inf or nothing above −inf has NaN in every
+ * value, its ids ordered with NaN first. top in [0, min(vocab, 64)]. */
+typedef struct {
+  int64_t bytes;
+  const void* logits;
+  int64_t ld, rows, vocab;
+  const int64_t* tokens;
+  int64_t top;
+  float *logprob, *entropy;
+  int64_t* top_ids;
+  float* top_logprobs;
+  int64_t dtype;
+} ssl_token_logprobs_args;
+int ssl_token_logprobs(const ssl_token_logprobs_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -183,6 +183,14 @@ class SlrStage(ctypes.Structure):
     ]
 
 
+# the paged entry points take one packed struct (paged.py, logprobs.py)
+for _name in ("ssl_paged_append", "ssl_paged_attention", "ssl_pages_free", "ssl_pages_fork",
+              "ssl_pages_compact", "ssl_token_logprobs"):
+    _SIGNATURES[_name] = (ctypes.c_int, [_c_p, _c_p])
+_SIGNATURES["ssl_paged_attention_workspace_size"] = (_c_i64, [_c_p])
+_SIGNATURES["ssl_pages_fork_workspace_size"] = (_c_i64, [_c_i64])
+_SIGNATURES["ssl_pages_compact_workspace_size"] = (_c_i64, [_c_i64])
+
 _SIGNATURES["ssl_slr_chain_sync_count"] = (_c_i64, [_c_i64])
 _SIGNATURES["ssl_slr_chain_frag_bytes"] = (_c_i64, [_c_i64, _c_i64])
 _SIGNATURES["ssl_slr_chain_table_bytes"] = (_c_i64, [])
