@@ -7,6 +7,8 @@
 
 namespace ssl {
 
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
 // Strides in elements. A page number read from the table is used only after
 // `has` accepted it.
 struct PagedCache {
@@ -26,5 +28,61 @@ struct PagedCache {
 // Checks `c` (the pools only where `pools`) and fills `out`.
 int paged_cache(const char* what, const ssl_paged_cache& c, int64_t struct_bytes, bool pools,
                 PagedCache* out);
+
+struct AttnArgs {
+  const char* q;
+  int64_t q_token, q_head;
+  char* out;  // [tokens, heads, head_dim]
+  const int32_t *lengths, *cu;
+  int64_t tokens;
+  int heads, window, sinks;
+  float scale_log2;  // scale · log2 e: scores are kept in base 2
+  // split contexts: the most parts of a row and its tiles per part at least,
+  // and the parts' outputs, maxima and sums
+  int n_split, per;
+  float *part_o, *part_ml;
+};
+
+// The positions a run of tokens at p_min … p_max of one sequence sees, as tiles
+// of T positions: the first `sink_tiles` of the context, then those from `base`.
+struct TileRange {
+  int sink_tiles, base, count;
+  __device__ __forceinline__ int tile(int i) const {
+    return i < sink_tiles ? i : i - sink_tiles + base;
+  }
+};
+template <int T>
+__device__ __forceinline__ TileRange tile_range(int p_min, int p_max, int window, int sinks) {
+  TileRange r{0, 0, 0};
+  if (p_max < 0) return r;
+  const int first = window && p_min + 1 > window ? p_min + 1 - window : 0;
+  r.base = first / T;
+  if (first > 0) r.sink_tiles = min((min(sinks, first) + T - 1) / T, r.base);
+  r.count = r.sink_tiles + p_max / T + 1 - r.base;
+  return r;
+}
+
+// The tiles a part of a row takes: A.per, or what spreads `count` over the
+// most parts. The kernels and the join compute the same.
+__device__ __forceinline__ int part_tiles(const AttnArgs& A, int count) {
+  return max(A.per, (count + A.n_split - 1) / A.n_split);
+}
+
+// Bits of two adjacent 16-bit elements, p rounded to nearest even.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+  if constexpr (DT == DT_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    bf16x2 v = {(__bf16)a, (__bf16)b};
+    return __builtin_bit_cast(uint32_t, v);
+  } else {
+    f16x2 v = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
+  }
+}
+
+// One token per sequence (paged_decode.hip), chunks (paged_prompt.hip).
+int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_length);
+int paged_decode_launch(const PagedCache& C, const AttnArgs& A, int dtype, hipStream_t st);
 
 }  // namespace ssl

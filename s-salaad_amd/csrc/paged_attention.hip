@@ -18,16 +18,6 @@
 namespace ssl {
 namespace {
 
-struct AttnArgs {
-  const char* q;
-  int64_t q_token, q_head;
-  char* out;
-  const int32_t *lengths, *cu;
-  int64_t tokens;
-  int heads, window, sinks;
-  float scale_log2;
-};
-
 // The token's sequence, by bisection of cu (the last s with cu[s] <= t; seqs
 // for tokens past the last).
 __device__ __forceinline__ int seq_of(const int32_t* cu, int seqs, int64_t t) {
@@ -115,38 +105,85 @@ void launch_rows(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
 
 using namespace ssl;
 
-extern "C" int64_t ssl_paged_attention_workspace_size(const ssl_paged_attention_args* a) {
-  (void)a;
-  return 0;
-}
+namespace ssl {
+namespace {
 
-extern "C" int ssl_paged_attention(const ssl_paged_attention_args* a, void* stream) {
-  clear_error();
+// Checks the arguments and fills the kernels' form of them; `need` receives the
+// workspace the call takes.
+int attention_args(const ssl_paged_attention_args* a, PagedCache* C, AttnArgs* A, int64_t* need) {
   const char* what = "paged_attention";
+  *need = 0;
   if (!a) return fail(SSL_ERR_INVALID, "%s: no arguments", what);
-  PagedCache C;
-  if (int rc = paged_cache(what, a->cache, sizeof(*a), true, &C)) return rc;
+  if (int rc = paged_cache(what, a->cache, sizeof(*a), true, C)) return rc;
   if (a->tokens < 0 || a->tokens > 0x7fffffff || a->heads <= 0 || a->heads > 65535 ||
-      a->heads % C.kv_heads)
+      a->heads % C->kv_heads)
     return fail(SSL_ERR_INVALID, "%s: %lld tokens, %lld heads over %d key/value heads", what,
-                (long long)a->tokens, (long long)a->heads, C.kv_heads);
-  if (a->window < 0 || a->sinks < 0)
-    return fail(SSL_ERR_INVALID, "%s: window %lld, sinks %lld", what, (long long)a->window,
-                (long long)a->sinks);
-  if (!a->cu && a->tokens != C.seqs)
+                (long long)a->tokens, (long long)a->heads, C->kv_heads);
+  if (a->window < 0 || a->sinks < 0 || a->max_tokens < 0 || a->max_length < 0)
+    return fail(SSL_ERR_INVALID, "%s: window %lld, sinks %lld, at most %lld tokens and %lld positions",
+                what, (long long)a->window, (long long)a->sinks, (long long)a->max_tokens,
+                (long long)a->max_length);
+  if (!a->cu && a->tokens != C->seqs)
     return fail(SSL_ERR_INVALID, "%s: %lld tokens for %d sequences", what, (long long)a->tokens,
-                C.seqs);
+                C->seqs);
   if (a->tokens == 0) return SSL_OK;
-  if (!a->q || !a->out || (!a->lengths && C.seqs))
+  if (!a->cu && a->tokens > 65535)
+    return fail(SSL_ERR_UNSUPPORTED, "%s: %lld sequences in one call (at most 65535)", what,
+                (long long)a->tokens);
+  if (!a->q || !a->out || (!a->lengths && C->seqs))
     return fail(SSL_ERR_INVALID, "%s: null pointer", what);
   const int64_t eb = elem_bytes((int)a->cache.dtype);
   if (!aligned(a->q, 16) || !aligned(a->out, 16) || (a->q_token * eb) % 16 || (a->q_head * eb) % 16)
     return fail(SSL_ERR_INVALID, "%s: q's rows and out must be 16-byte aligned", what);
-  AttnArgs A{(const char*)a->q, a->q_token, a->q_head, (char*)a->out, a->lengths, a->cu, a->tokens,
-             (int)a->heads, (int)std::min<int64_t>(a->window, 0x7fffffff),
-             (int)std::min<int64_t>(a->sinks, 0x7fffffff), (float)(a->scale * 1.4426950408889634)};
-  if (a->cache.dtype == SSL_F32) launch_rows<DT_F32>(C, A, (hipStream_t)stream);
-  else if (a->cache.dtype == SSL_BF16) launch_rows<DT_BF16>(C, A, (hipStream_t)stream);
-  else launch_rows<DT_F16>(C, A, (hipStream_t)stream);
+  // lane offsets within a page's head are 32-bit
+  if (C->page * C->slot_stride * eb > 0x7fffffff)
+    return fail(SSL_ERR_UNSUPPORTED, "%s: a page's head spans 2 GiB or more", what);
+  *A = AttnArgs{};
+  A->q = (const char*)a->q;
+  A->q_token = a->q_token;
+  A->q_head = a->q_head;
+  A->out = (char*)a->out;
+  A->lengths = a->lengths;
+  A->cu = a->cu;
+  A->tokens = a->tokens;
+  A->heads = (int)a->heads;
+  // positions are below 2^31, so larger values mean the same as these
+  A->window = (int)std::min<int64_t>(a->window, 0x7fffffff);
+  A->sinks = (int)std::min<int64_t>(a->sinks, 0x7fffffff);
+  A->scale_log2 = (float)(a->scale * 1.4426950408889634);
+  const int64_t reach = std::min<int64_t>(a->max_length, (int64_t)C->cols * C->page);
+  if (!a->cu && C->cols) *need = paged_decode_plan(*C, A, (int)a->cache.dtype, reach);
+  return SSL_OK;
+}
+
+}  // namespace
+}  // namespace ssl
+
+extern "C" int64_t ssl_paged_attention_workspace_size(const ssl_paged_attention_args* a) {
+  PagedCache C;
+  AttnArgs A;
+  int64_t need;
+  return attention_args(a, &C, &A, &need) == SSL_OK ? need : 0;
+}
+
+extern "C" int ssl_paged_attention(const ssl_paged_attention_args* a, void* stream) {
+  clear_error();
+  PagedCache C;
+  AttnArgs A;
+  int64_t need;
+  if (int rc = attention_args(a, &C, &A, &need)) return rc;
+  if (a->tokens == 0) return SSL_OK;
+  if (need) {
+    if (!a->workspace || a->workspace_bytes < need || !aligned(a->workspace, 16))
+      return fail(SSL_ERR_WORKSPACE, "paged_attention: workspace of %lld bytes needed",
+                  (long long)need);
+    A.part_o = (float*)a->workspace;
+    A.part_ml = A.part_o + need / 4 / (C.head_dim + 2) * C.head_dim;
+  }
+  hipStream_t st = (hipStream_t)stream;
+  if (!a->cu && C.cols) return paged_decode_launch(C, A, (int)a->cache.dtype, st);
+  if (a->cache.dtype == SSL_F32) launch_rows<DT_F32>(C, A, st);
+  else if (a->cache.dtype == SSL_BF16) launch_rows<DT_BF16>(C, A, st);
+  else launch_rows<DT_F16>(C, A, st);
   return check_hip(hipGetLastError(), "paged_attention launch");
 }
