@@ -36,7 +36,10 @@ struct AttnArgs {
   const int32_t *lengths, *cu;
   int64_t tokens;
   int heads, window, sinks;
-  float scale_log2;  // scale · log2 e: scores are kept in base 2
+  // |scale| · log2 e (scores are kept in base 2; 1 for a scale of 0), and what
+  // its sign does to q: kept bits, flipped sign bits
+  float scale_log2;
+  uint32_t keep, flip;
   // split contexts: the most parts of a row and its tiles per part at least,
   // and the parts' outputs, maxima and sums
   int n_split, per;
@@ -84,5 +87,9 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 // One token per sequence (paged_decode.hip), chunks (paged_prompt.hip).
 int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_length);
 int paged_decode_launch(const PagedCache& C, const AttnArgs& A, int dtype, hipStream_t st);
+int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
+                          int64_t max_length);
+int paged_prompt_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64_t max_tokens,
+                        hipStream_t st);
 
 }  // namespace ssl

@@ -84,6 +84,13 @@ __global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode
         A.q, s * A.q_token + (int64_t)(h0 + min(c, rows - 1)) * A.q_head + (4 * i + g) * S::KE,
         S::KE);
 
+  {
+    uint32_t* q = (uint32_t*)qf;
+    const uint32_t flip = A.flip & (DT == DT_F32 ? 0x80000000u : 0x80008000u);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof qf / 4); ++i) q[i] = (q[i] & A.keep) ^ flip;
+  }
+
   // lane offsets within a page's head: key c for K, keys 4g + e for V
   const uint32_t slot_bytes = (uint32_t)(C.slot_stride * S::EB);
   const uint32_t k_off = c * slot_bytes + g * S::KE * S::EB;

@@ -1,0 +1,583 @@
+// Attention of chunks of tokens over their sequences' pages: causal, with an
+// optional window and first tokens that stay visible.
+//
+// 4·head_dim operations a (token, visible position, head): the matrix cores
+// bound it. A row is one query head of one token; the rows of a key/value head
+// are packed token by token (row r: token r / G, head r % G of the group), so
+// short chunks of grouped heads fill the tiles and share what is loaded. A
+// wave holds 32 rows, four waves (a team) 128; the teams of a workgroup take
+// alternate tiles of KT positions and are joined through LDS.
+//
+//   Sᵀ = K·Qᵀ    32 keys × 32 rows a matrix instruction; a lane holds 16 keys of
+//                one row, so its softmax needs one exchange between lane halves
+//                and the running maximum and sum are scalars of a lane.
+//   Oᵀ = Vᵀ·Pᵀ   P as the accumulators leave it (a contraction may take the keys
+//                in any order both operands share); V is transposed on its way
+//                out of LDS (ds_read_tr16), fp32 values are read as they are.
+//
+// K and V go from memory into LDS directly, a tile ahead of its use, two
+// buffers a team, one barrier a tile. LDS rows are permuted in 16-byte chunks by
+// the row, so that fragment reads spread over the banks; the permutation is made
+// by the address each lane loads. What lies past the last visible position or on
+// no page is filled with zeros by the loads' bounds.
+#include <hip/hip_runtime.h>
+#include <math.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "paged.h"
+
+namespace ssl {
+namespace {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <int DT, int HD>
+struct Tile {
+  static constexpr int EB = Elem<DT>::bytes;
+  static constexpr bool F32 = DT == DT_F32;
+  static constexpr int TEAMS = HD == 256 ? 1 : 2;
+  static constexpr int KT = F32 ? 32 : 64;      // positions a tile
+  static constexpr int ROWS = 128;              // rows a workgroup
+  static constexpr int RB = HD * EB;            // bytes of an LDS row
+  static constexpr int CPR = RB / 16;           // 16-byte chunks of a row
+  static constexpr int RI = 1024 / RB;          // rows one load instruction fills
+  static constexpr int IPG = 16 / RI;           // instructions a group of 16 rows
+  static constexpr int NQ = IPG / 4 > 0 ? IPG / 4 : 1;
+  static constexpr int BUF = KT * RB;           // one of K, V
+  static constexpr int LDS = TEAMS * 4 * BUF;
+  static constexpr int THREADS = TEAMS * 256;
+  static constexpr int KS = KT / 32;
+  static constexpr int QS = HD / (F32 ? 8 : 16);  // contraction steps of Sᵀ
+  static constexpr int OT = HD / 32;              // output tiles
+  // the chunk permutation of row r (of a group of 16)
+  __device__ static int swz_k(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
+  __device__ static int swz_v(int r) { return F32 ? 0 : CPR == 8 ? r & 6 : (r & 7) << 1; }
+};
+
+// 16 bytes a lane from memory into LDS (lane l: lds + 16·l), zeros past the
+// resource's size. In assembly, so that the compiler adds no waits of its own
+// for it: wait_loads and the barrier below order it.
+__device__ __forceinline__ void dma16(const u32x4& r, uint32_t voff, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(r)
+               : "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+__device__ __forceinline__ uint32_t lds_addr(const void* p) {
+  return __builtin_amdgcn_readfirstlane(
+      (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p);
+}
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// 4 elements of column l % 16 of the 4 × 16 block a group of 16 lanes addresses
+// (lane l: row l / 4, 4 elements from 4·(l % 4))
+__device__ __forceinline__ uint2 read_tr(uint32_t lds) {
+  return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4*)(uintptr_t)lds));
+}
+__device__ __forceinline__ uint4 read16(uint32_t lds) {
+  return __builtin_bit_cast(uint4, *(__attribute__((address_space(3))) u32x4*)(uintptr_t)lds);
+}
+__device__ __forceinline__ uint2 read8(uint32_t lds) {
+  return __builtin_bit_cast(uint2, *(__attribute__((address_space(3))) u32x2*)(uintptr_t)lds);
+}
+
+template <int DT>
+__device__ __forceinline__ void mma(f32x16& acc, const uint4& a, const uint4& b) {
+  if constexpr (DT == DT_BF16)
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                  __builtin_bit_cast(bf16x8, b), acc, 0, 0, 0);
+  else
+    acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                 __builtin_bit_cast(f16x8, b), acc, 0, 0, 0);
+}
+__device__ __forceinline__ void mma_f32(f32x16& acc, float a, float b) {
+  acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, acc, 0, 0, 0);
+}
+
+// A sequence's rows of one key/value head and their positions.
+struct Chunk {
+  int64_t t0;  // its first token
+  int rows, p0;  // p0: the first token's position
+  __device__ __forceinline__ Chunk(const PagedCache& C, const AttnArgs& A, int s, int G) {
+    int64_t a = s == 0 ? 0 : A.cu[s], b = A.cu[s + 1];
+    a = min(max(a, (int64_t)0), A.tokens);
+    b = min(max(b, a), A.tokens);
+    t0 = a;
+    rows = (int)(b - a) * G;
+    p0 = min(max(A.lengths[s], 0), C.cols << C.log2_page) - (int)(b - a);
+  }
+};
+
+template <int DT, int HD>
+__global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCache C, AttnArgs A,
+                                                                          int n_tiles) {
+  using T = Tile<DT, HD>;
+  extern __shared__ char lds[];
+  const int G = A.heads / C.kv_heads;
+  // key/value heads fastest (one head's K and V stay in one die's cache where
+  // their number is a multiple of 8), the longest rows' tiles first
+  uint32_t id = blockIdx.x;
+  const int kh = id % C.kv_heads;
+  id /= C.kv_heads;
+  const int split = id % A.n_split;
+  id /= A.n_split;
+  const int s = id % (C.seqs + 1);
+  const int tile0 = n_tiles - 1 - (int)(id / (C.seqs + 1));
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int team = wave >> 2, w = wave & 3;
+  const int col = lane & 31, h = lane >> 5;
+
+  if (s == C.seqs) {  // tokens past the last chunk
+    if (tile0 || split) return;
+    const int64_t end = min(max((int64_t)A.cu[s], (int64_t)0), A.tokens);
+    const int64_t n = (A.tokens - end) * G * T::CPR;
+    for (int64_t i = tid; i < n; i += T::THREADS) {
+      const int64_t r = i / T::CPR;
+      *(uint4*)(A.out + (((end + r / G) * A.heads + kh * G + r % G) * T::CPR + i % T::CPR) * 16) =
+          uint4{0, 0, 0, 0};
+    }
+    return;
+  }
+  const Chunk chunk(C, A, s, G);
+  const int32_t* table = C.table + (int64_t)s * C.table_stride;
+  const uint32_t slot_bytes = (uint32_t)(C.slot_stride * T::EB);
+  constexpr float kBias = DT == DT_F16 ? 4.f : 0.f;  // fp16 weights are kept 16-fold
+
+  for (int tile = tile0; tile * T::ROWS < chunk.rows; tile += n_tiles) {
+    const int row_a = tile * T::ROWS, row_b = min(row_a + T::ROWS, chunk.rows) - 1;
+    const int p_min = chunk.p0 + row_a / G, p_max = chunk.p0 + row_b / G;
+    const TileRange range = tile_range<T::KT>(max(p_min, 0), p_max, A.window, A.sinks);
+    const int per = part_tiles(A, range.count);
+    const bool whole = per >= range.count;
+    const int lo = split * per, hi = min(lo + per, range.count);
+    if (lo >= hi && split > 0) continue;
+    const int limit = p_max + 1;
+    const int w_first = A.window && p_min + 1 > A.window ? p_min + 1 - A.window : 0;
+
+    // this wave's rows
+    const int r_a = row_a + w * 32;
+    const bool any = r_a <= row_b;
+    const int r = min(r_a + col, row_b);
+    const int64_t token = chunk.t0 + r / G;
+    const int head = kh * G + r % G;
+    const int p = chunk.p0 + r / G;
+    const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
+    const int wp_min = chunk.p0 + r_a / G, wp_max = chunk.p0 + min(r_a + 31, row_b) / G;
+    const int wfirst_min = A.window && wp_min + 1 > A.window ? wp_min + 1 - A.window : 0;
+    const int wfirst_max = A.window && wp_max + 1 > A.window ? wp_max + 1 - A.window : 0;
+
+    uint4 qf[T::QS];
+#pragma unroll
+    for (int i = 0; i < T::QS; ++i) {
+      qf[i] = *(const uint4*)(A.q + (token * A.q_token + (int64_t)head * A.q_head) * T::EB +
+                              (2 * i + h) * 16);
+      const uint32_t flip = A.flip & (T::F32 ? 0x80000000u : 0x80008000u);
+      qf[i] = uint4{(qf[i].x & A.keep) ^ flip, (qf[i].y & A.keep) ^ flip,
+                    (qf[i].z & A.keep) ^ flip, (qf[i].w & A.keep) ^ flip};
+    }
+    f32x16 o[T::OT];
+#pragma unroll
+    for (int i = 0; i < T::OT; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+    float m = -INFINITY, l = 0.f;
+
+    const uint32_t lds0 = lds_addr(lds) + team * 4 * T::BUF;
+    // load lanes: LDS chunk lane % CPR of row lane / CPR of an instruction
+    uint32_t k_off[T::NQ], v_off[T::NQ];
+    int l_row[T::NQ];
+#pragma unroll
+    for (int q = 0; q < T::NQ; ++q) {
+      const int r16 = (T::IPG >= 4 ? (q * 4 + w) * T::RI : (w & 1) * T::RI) + lane / T::CPR;
+      l_row[q] = r16;
+      k_off[q] = r16 * slot_bytes + ((lane % T::CPR) ^ T::swz_k(r16)) * 16;
+      v_off[q] = r16 * slot_bytes + ((lane % T::CPR) ^ T::swz_v(r16)) * 16;
+    }
+    // page of group lane % (KT / 16) of tile i
+    auto pages_of = [&](int i) {
+      const int key = range.tile(min(i, hi - 1)) * T::KT + 16 * (lane % (T::KT / 16));
+      return table[min(key >> C.log2_page, C.cols - 1)];
+    };
+    auto load_tile = [&](int i, int buf, int32_t pgv) {
+      const int key0 = range.tile(i) * T::KT;
+      const bool below = key0 < w_first && key0 + T::KT > A.sinks;
+#pragma unroll
+      for (int n = 0; n < (T::IPG >= 4 ? T::KT / 16 : T::KT / 32); ++n) {
+        const int grp = T::IPG >= 4 ? n : 2 * n + (w >> 1);
+        const int32_t page = __builtin_amdgcn_readlane(pgv, grp);
+        const int key = key0 + 16 * grp;
+        const int rows = C.has(page) ? min(max(limit - key, 0), 16) : 0;
+        const int64_t off = ((rows ? page : 0) * C.page_stride + kh * C.head_stride +
+                             (key & (C.page - 1)) * C.slot_stride) * T::EB;
+        u32x4 rk, rv;
+        const uint64_t ka = (uint64_t)(uintptr_t)(C.k + off), va = (uint64_t)(uintptr_t)(C.v + off);
+        rk[0] = __builtin_amdgcn_readfirstlane((uint32_t)ka);
+        rk[1] = __builtin_amdgcn_readfirstlane((uint32_t)(ka >> 32) & 0xffffu);
+        rv[0] = __builtin_amdgcn_readfirstlane((uint32_t)va);
+        rv[1] = __builtin_amdgcn_readfirstlane((uint32_t)(va >> 32) & 0xffffu);
+        rk[2] = rv[2] = __builtin_amdgcn_readfirstlane(rows * slot_bytes);
+        rk[3] = rv[3] = 0x00020000u;
+#pragma unroll
+        for (int q = 0; q < T::NQ; ++q) {
+          const int base = 16 * grp + (T::IPG >= 4 ? (q * 4 + w) * T::RI : (w & 1) * T::RI);
+          uint32_t hide = 0;  // positions before the window: zeros as well
+          if (below) {
+            const int kk = key + l_row[q];
+            hide = kk < w_first && kk >= A.sinks ? 0x80000000u : 0u;
+          }
+          dma16(rk, k_off[q] | hide, lds0 + (2 * buf) * T::BUF + base * T::RB);
+          dma16(rv, v_off[q] | hide, lds0 + (2 * buf + 1) * T::BUF + base * T::RB);
+        }
+      }
+    };
+
+    // fragment addresses within a buffer
+    const uint32_t ka = col * T::RB + (h ^ T::swz_k(col & 15)) * 16;
+    uint32_t va;
+    if constexpr (T::F32)
+      va = 4 * h * T::RB + col * (HD == 64 ? 8 : 16);
+    else
+      va = (4 * h + ((lane & 15) >> 2)) * T::RB + (lane & 3) * 8 +
+           ((((lane >> 4) & 1) ^ (T::swz_v(4 * h + ((lane & 15) >> 2)) >> 1)) * 32);
+
+    const int rounds = (hi - lo + T::TEAMS - 1) / T::TEAMS;
+    int32_t pgv = 0;
+    uint32_t bad = 0, bad_next = 0;  // groups of 16 of the tile that lie on no page
+    auto missing = [&](int32_t pg) {
+      return (uint32_t)__ballot(!C.has(pg)) & ((1u << (T::KT / 16)) - 1);
+    };
+    barrier();  // the rows before have left the buffers
+    if (lo + team < hi) {
+      pgv = pages_of(lo + team);
+      bad_next = missing(pgv);
+      load_tile(lo + team, 0, pgv);
+    }
+    pgv = lo + team + T::TEAMS < hi ? pages_of(lo + team + T::TEAMS) : 0;
+    for (int n = 0; n < rounds; ++n) {
+      const int i = lo + n * T::TEAMS + team;
+      wait_loads();
+      barrier();
+      bad = bad_next;
+      if (i + T::TEAMS < hi) {
+        bad_next = missing(pgv);
+        load_tile(i + T::TEAMS, (n + 1) & 1, pgv);
+        pgv = pages_of(i + 2 * T::TEAMS);
+      }
+      if (i >= hi || !any) continue;
+      const int key0 = range.tile(i) * T::KT;
+      // nothing of it is seen by the wave
+      if (key0 > wp_max || (key0 + T::KT <= wfirst_min && key0 >= A.sinks)) continue;
+      const uint32_t kb = lds0 + 2 * (n & 1) * T::BUF, vb = kb + T::BUF;
+
+      f32x16 x[T::KS];
+#pragma unroll
+      for (int t = 0; t < T::KS; ++t) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] = 0.f;
+#pragma unroll
+        for (int k = 0; k < T::QS; ++k) {
+          const uint4 kf = read16(kb + (ka ^ (k * 32)) + t * 32 * T::RB);
+          if constexpr (T::F32) {
+            mma_f32(x[t], __uint_as_float(kf.x), __uint_as_float(qf[k].x));
+            mma_f32(x[t], __uint_as_float(kf.y), __uint_as_float(qf[k].y));
+            mma_f32(x[t], __uint_as_float(kf.z), __uint_as_float(qf[k].z));
+            mma_f32(x[t], __uint_as_float(kf.w), __uint_as_float(qf[k].w));
+          } else {
+            mma<DT>(x[t], kf, qf[k]);
+          }
+        }
+      }
+      const bool all = key0 + T::KT - 1 <= wp_min && !bad &&
+                       (key0 >= wfirst_max || key0 + T::KT <= A.sinks);
+      if (!all) {
+#pragma unroll
+        for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = key0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+            const bool see = key <= p && (key >= first || key < A.sinks) &&
+                             !((bad >> (2 * t + (e >> 3))) & 1);
+            x[t][e] = see ? x[t][e] : -INFINITY;
+          }
+      }
+      float mx = x[0][0];
+#pragma unroll
+      for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32)) * A.scale_log2;
+      // o and l keep an older maximum while it is at most 2^8 too small: the
+      // weights stay in range and most tiles need no scaling
+      if (__any(mx > m + 8.f)) {
+        const float top = fmaxf(m, mx);
+        const float a = exp2f(m - (top == -INFINITY ? 0.f : top));
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < T::OT; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= a;
+        m = top;
+      }
+      const float base = (m == -INFINITY ? 0.f : m) - kBias;
+      float sum = 0.f;
+#pragma unroll
+      for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          x[t][e] = __builtin_amdgcn_exp2f(fmaf(x[t][e], A.scale_log2, -base));
+          sum += x[t][e];
+        }
+      l += sum;
+      if constexpr (T::F32) {
+#pragma unroll
+        for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t at = vb + va + (32 * t + 8 * (e >> 2) + (e & 3)) * T::RB;
+            if constexpr (HD == 64) {
+              const uint2 v = read8(at);
+              mma_f32(o[0], __uint_as_float(v.x), x[t][e]);
+              mma_f32(o[1], __uint_as_float(v.y), x[t][e]);
+            } else {
+#pragma unroll
+              for (int d = 0; d < T::OT; d += 4) {
+                const uint4 v = read16(at + d * 128);
+                mma_f32(o[d], __uint_as_float(v.x), x[t][e]);
+                mma_f32(o[d + 1], __uint_as_float(v.y), x[t][e]);
+                mma_f32(o[d + 2], __uint_as_float(v.z), x[t][e]);
+                mma_f32(o[d + 3], __uint_as_float(v.w), x[t][e]);
+              }
+            }
+          }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2 * T::KS; ++j) {
+          const int e = 8 * (j & 1);
+          const f32x16& y = x[j >> 1];
+          const uint4 pf = {pack2<DT>(y[e], y[e + 1]), pack2<DT>(y[e + 2], y[e + 3]),
+                            pack2<DT>(y[e + 4], y[e + 5]), pack2<DT>(y[e + 6], y[e + 7])};
+#pragma unroll
+          for (int d = 0; d < T::OT; ++d) {
+            const uint32_t at = vb + (va ^ (d * 64)) + 16 * j * T::RB;
+            const uint2 a = read_tr(at), b = read_tr(at + 8 * T::RB);
+            mma<DT>(o[d], uint4{a.x, a.y, b.x, b.y}, pf);
+          }
+        }
+      }
+    }
+    l += __shfl_xor(l, 32);
+
+    // the second team's part joins the first's
+    if constexpr (T::TEAMS == 2) {
+      barrier();
+      f32x4* part = (f32x4*)lds;
+      float* ml = (float*)(lds + 4 * T::OT * 4 * 64 * 16);
+      if (team == 1) {
+#pragma unroll
+        for (int d = 0; d < T::OT; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            part[((w * T::OT + d) * 4 + k) * 64 + lane] =
+                f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
+        ml[(w * 2) * 64 + lane] = m;
+        ml[(w * 2 + 1) * 64 + lane] = l;
+      }
+      barrier();
+      if (team == 1) continue;
+      const float m2 = ml[(w * 2) * 64 + lane], l2 = ml[(w * 2 + 1) * 64 + lane];
+      const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+      const float a = exp2f(m - base), b = exp2f(m2 - base);
+      l = l * a + l2 * b;
+      m = top;
+#pragma unroll
+      for (int d = 0; d < T::OT; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const f32x4 y = part[((w * T::OT + d) * 4 + k) * 64 + lane];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[d][4 * k + e] = o[d][4 * k + e] * a + y[e] * b;
+        }
+    }
+    if (r_a + col > row_b) continue;
+    const int64_t at = token * A.heads + head;
+    float inv = 1.f;
+    if (whole) {
+      inv = l == 0.f ? 0.f : 1.f / l;
+    } else if (h == 0) {
+      float* ml = A.part_ml + 2 * (at * A.n_split + split);
+      ml[0] = m;
+      ml[1] = l;
+    }
+    // 4 adjacent features at a time (fp32, 64 wide: 2)
+    auto put = [&](int f, const f32x4 y) {
+      if (!whole)
+        *(f32x4*)(A.part_o + (at * A.n_split + split) * HD + f) = y;
+      else if constexpr (T::F32)
+        *(f32x4*)(A.out + (at * HD + f) * 4) = y;
+      else
+        *(uint2*)(A.out + (at * HD + f) * 2) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+    };
+    if constexpr (!T::F32) {
+#pragma unroll
+      for (int d = 0; d < T::OT; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          put(32 * d + 8 * k + 4 * h, f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2],
+                                            o[d][4 * k + 3]} * inv);
+    } else if constexpr (HD > 64) {
+#pragma unroll
+      for (int d = 0; d < T::OT; d += 4)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          put(32 * d + 4 * (8 * (e >> 2) + 4 * h + (e & 3)),
+              f32x4{o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]} * inv);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 16; e += 2)
+        put(2 * (8 * (e >> 2) + 4 * h + (e & 3)),
+            f32x4{o[0][e], o[1][e], o[0][e + 1], o[1][e + 1]} * inv);
+    }
+  }
+}
+
+// The parts of split rows joined, a wave a row.
+template <int DT, int HD>
+__global__ __launch_bounds__(256) void prompt_join_kernel(PagedCache C, AttnArgs A) {
+  using T = Tile<DT, HD>;
+  constexpr int LN = HD / 4, NG = 64 / LN;
+  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
+  const int64_t t = at / A.heads;
+  if (t >= A.tokens) return;
+  int a = 0, b = C.seqs;  // the sequence: the first whose end lies past t
+  while (a < b) {
+    const int mid = (a + b) >> 1;
+    if (A.cu[mid + 1] > t) b = mid;
+    else a = mid + 1;
+  }
+  if (a >= C.seqs) return;
+  const int G = A.heads / C.kv_heads;
+  const Chunk chunk(C, A, a, G);
+  const int r = (int)(t - chunk.t0) * G + (int)(at % A.heads) % G;
+  if (r < 0 || r >= chunk.rows) return;
+  const int row_a = r / T::ROWS * T::ROWS, row_b = min(row_a + T::ROWS, chunk.rows) - 1;
+  const TileRange range = tile_range<T::KT>(max(chunk.p0 + row_a / G, 0), chunk.p0 + row_b / G,
+                                            A.window, A.sinks);
+  const int per = part_tiles(A, range.count);
+  if (per >= range.count) return;
+  const int parts = (range.count + per - 1) / per;
+  const int d = lane % LN, grp = lane / LN;
+  const float* ml = A.part_ml + 2 * at * A.n_split;
+  const float* po = A.part_o + at * A.n_split * HD + 4 * d;
+  float top = -INFINITY;
+  for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[2 * i]);
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
+  const float base = top == -INFINITY ? 0.f : top;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  for (int i = grp; i < parts; i += NG) {
+    const float x = exp2f(ml[2 * i] - base);
+    sum += ml[2 * i + 1] * x;
+    acc += *(const f32x4*)(po + (int64_t)i * HD) * x;
+  }
+#pragma unroll
+  for (int o = LN; o < 64; o <<= 1) {
+    sum += __shfl_xor(sum, o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
+  }
+  if (grp) return;
+  acc *= sum == 0.f ? 0.f : 1.f / sum;
+  if constexpr (DT == DT_F32)
+    *(f32x4*)(A.out + (at * HD + 4 * d) * 4) = acc;
+  else
+    *(uint2*)(A.out + (at * HD + 4 * d) * 2) =
+        uint2{pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3])};
+}
+
+int64_t row_tiles(const AttnArgs& A, int G, int64_t max_tokens) {
+  return std::max<int64_t>(1, (max_tokens * G + 127) / 128);
+}
+
+template <int DT, int HD>
+int launch(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
+  using T = Tile<DT, HD>;
+  const int64_t n_tiles = row_tiles(A, A.heads / C.kv_heads, max_tokens);
+  const int64_t grid = n_tiles * (C.seqs + 1) * A.n_split * C.kv_heads;
+  if (grid > 0x7fffffff)
+    return fail(SSL_ERR_UNSUPPORTED, "paged_attention: a grid of %lld workgroups", (long long)grid);
+  if (T::LDS > 64 * 1024) {
+    static bool raised[64] = {};  // per device
+    int dev = 0;
+    if (int rc = check_hip(hipGetDevice(&dev), "device query")) return rc;
+    if (dev < 0 || dev >= 64 || !raised[dev]) {
+      if (int rc = check_hip(hipFuncSetAttribute((const void*)prompt_kernel<DT, HD>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS),
+                             "shared memory size"))
+        return rc;
+      if (dev >= 0 && dev < 64) raised[dev] = true;
+    }
+  }
+  hipLaunchKernelGGL((prompt_kernel<DT, HD>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS, st, C,
+                     A, (int)n_tiles);
+  if (A.n_split > 1) {
+    const int64_t rows = A.tokens * A.heads;
+    hipLaunchKernelGGL((prompt_join_kernel<DT, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
+                       st, C, A);
+  }
+  return SSL_OK;
+}
+
+template <int DT>
+int launch_dt(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
+  if (C.head_dim == 64) return launch<DT, 64>(C, A, max_tokens, st);
+  if (C.head_dim == 128) return launch<DT, 128>(C, A, max_tokens, st);
+  return launch<DT, 256>(C, A, max_tokens, st);
+}
+
+}  // namespace
+
+// Contexts are split where the rows' tiles do not fill the device, into parts
+// of 4 tiles at least. Fills n_split and per; returns the parts' bytes.
+int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
+                          int64_t max_length) {
+  const int KT = dtype == SSL_F32 ? 32 : 64;
+  const int G = A->heads / C.kv_heads;
+  const int64_t tiles = std::min<int64_t>(C.seqs * row_tiles(*A, G, max_tokens),
+                                          A->tokens * G / 128 + C.seqs);
+  const int64_t blocks = std::max<int64_t>(1, tiles * C.kv_heads);
+  int64_t reach = max_length;
+  if (A->window)
+    reach = std::min<int64_t>(reach, (int64_t)A->window + std::min(A->sinks, 0x3fffffff) +
+                                         128 / G + 2 * KT);
+  const int64_t keys = std::max<int64_t>(1, (reach + KT - 1) / KT);
+  const int64_t want = std::max<int64_t>(1, 512 / blocks);
+  const int64_t per = std::max<int64_t>(4, (keys + want - 1) / want);
+  A->per = (int)std::min<int64_t>(per, 0x3fffffff);
+  A->n_split = (int)std::max<int64_t>(1, std::min<int64_t>((keys + per - 1) / per, 65535));
+  if (A->n_split <= 1) return 0;
+  return A->tokens * A->heads * (int64_t)A->n_split * (C.head_dim + 2) * 4;
+}
+
+int paged_prompt_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64_t max_tokens,
+                        hipStream_t st) {
+  int rc;
+  if (dtype == SSL_F32) rc = launch_dt<DT_F32>(C, A, max_tokens, st);
+  else if (dtype == SSL_BF16) rc = launch_dt<DT_BF16>(C, A, max_tokens, st);
+  else rc = launch_dt<DT_F16>(C, A, max_tokens, st);
+  return rc ? rc : check_hip(hipGetLastError(), "paged prompt attention launch");
+}
+
+}  // namespace ssl
