@@ -124,22 +124,26 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   extern __shared__ char lds[];
   const int G = A.heads / C.kv_heads;
   // key/value heads fastest (one head's K and V stay in one die's cache where
-  // their number is a multiple of 8), the longest rows' tiles first
+  // their number is a multiple of 8), the longest rows' tiles first; then a
+  // workgroup a head for the tokens past the last chunk. (Between the others
+  // those, which end at once, would leave shader engines idle: workgroups go to
+  // the engines in turn.)
   uint32_t id = blockIdx.x;
   const int kh = id % C.kv_heads;
   id /= C.kv_heads;
   const int split = id % A.n_split;
   id /= A.n_split;
-  const int s = id % (C.seqs + 1);
-  const int tile0 = n_tiles - 1 - (int)(id / (C.seqs + 1));
+  const bool tail = id >= (uint32_t)n_tiles * C.seqs;
+  const int s = tail ? C.seqs : id % C.seqs;
+  const int tile0 = tail ? 0 : n_tiles - 1 - (int)(id / C.seqs);
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int team = wave >> 2, w = wave & 3;
   const int col = lane & 31, h = lane >> 5;
 
-  if (s == C.seqs) {  // tokens past the last chunk
-    if (tile0 || split) return;
+  if (tail) {
+    if (split) return;
     const int64_t end = min(max((int64_t)A.cu[s], (int64_t)0), A.tokens);
     const int64_t n = (A.tokens - end) * G * T::CPR;
     for (int64_t i = tid; i < n; i += T::THREADS) {
@@ -515,7 +519,7 @@ template <int DT, int HD>
 int launch(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
   using T = Tile<DT, HD>;
   const int64_t n_tiles = row_tiles(A, A.heads / C.kv_heads, max_tokens);
-  const int64_t grid = n_tiles * (C.seqs + 1) * A.n_split * C.kv_heads;
+  const int64_t grid = (n_tiles * C.seqs + 1) * A.n_split * C.kv_heads;
   if (grid > 0x7fffffff)
     return fail(SSL_ERR_UNSUPPORTED, "paged_attention: a grid of %lld workgroups", (long long)grid);
   if (T::LDS > 64 * 1024) {
