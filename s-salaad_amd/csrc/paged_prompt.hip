@@ -25,6 +25,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <utility>
 
 #include "paged.h"
 
@@ -58,14 +59,15 @@ struct Tile {
   __device__ static int swz_v(int r) { return F32 ? 0 : CPR == 8 ? r & 6 : (r & 7) << 1; }
 };
 
-// 16 bytes a lane from memory into LDS (lane l: lds + 16·l), zeros past the
+// 16 bytes a lane from memory into LDS (lane l: lds + OFF + 16·l), zeros past the
 // resource's size. In assembly, so that the compiler adds no waits of its own
 // for it: wait_loads and the barrier below order it.
+template <int OFF>
 __device__ __forceinline__ void dma16(const u32x4& r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_add_u32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
-               : "s"(lds), "v"(voff), "s"(r)
-               : "m0");
+               : "s"(lds), "v"(voff), "s"(r), "n"(OFF)
+               : "m0", "scc");
 }
 __device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 __device__ __forceinline__ void barrier() {
@@ -101,6 +103,15 @@ __device__ __forceinline__ void mma(f32x16& acc, const uint4& a, const uint4& b)
 }
 __device__ __forceinline__ void mma_f32(f32x16& acc, float a, float b) {
   acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, acc, 0, 0, 0);
+}
+
+template <typename F, int... I>
+__device__ __forceinline__ void unroll_over(F& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unroll(F f) {
+  unroll_over(f, std::make_integer_sequence<int, N>{});
 }
 
 // A sequence's rows of one key/value head and their positions.
@@ -156,6 +167,9 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   const Chunk chunk(C, A, s, G);
   const int32_t* table = C.table + (int64_t)s * C.table_stride;
   const uint32_t slot_bytes = (uint32_t)(C.slot_stride * T::EB);
+  const uint64_t page_bytes = (uint64_t)C.page_stride * T::EB;
+  const uint64_t k_base = (uint64_t)(uintptr_t)C.k + kh * C.head_stride * T::EB;
+  const uint64_t v_base = (uint64_t)(uintptr_t)C.v + kh * C.head_stride * T::EB;
   constexpr float kBias = DT == DT_F16 ? 4.f : 0.f;  // fp16 weights are kept 16-fold
 
   for (int tile = tile0; tile * T::ROWS < chunk.rows; tile += n_tiles) {
@@ -213,47 +227,201 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
       const int key = range.tile(min(i, hi - 1)) * T::KT + 16 * (lane % (T::KT / 16));
       return table[min(key >> C.log2_page, C.cols - 1)];
     };
-    auto load_tile = [&](int i, int buf, int32_t pgv) {
+    // Each lane settles one group of 16 positions (group lane % (KT / 16)): its
+    // place in the pools and the bytes of it that are loaded; the loads then read
+    // theirs from that lane.
+    auto load_tile = [&](int i, int buf, int32_t page) {
+      constexpr int KG = T::KT / 16;
       const int key0 = range.tile(i) * T::KT;
+      const int key_l = key0 + 16 * (lane % KG);
+      const bool has = C.has(page);
+      const uint64_t off_l = (uint64_t)(uint32_t)(has ? page : 0) * page_bytes +
+                             (uint32_t)(key_l & (C.page - 1)) * slot_bytes;
+      const uint32_t size_l = has ? min(max(limit - key_l, 0), 16) * slot_bytes : 0u;
       const bool below = key0 < w_first && key0 + T::KT > A.sinks;
-#pragma unroll
-      for (int n = 0; n < (T::IPG >= 4 ? T::KT / 16 : T::KT / 32); ++n) {
+      // instruction (n, q) fills 1 KiB at n · max(IPG, 4) + 4 q + w
+      const uint32_t to = lds0 + 2 * buf * T::BUF + w * 1024;
+      unroll<(T::IPG >= 4 ? KG : KG / 2)>([&](auto n) {
         const int grp = T::IPG >= 4 ? n : 2 * n + (w >> 1);
-        const int32_t page = __builtin_amdgcn_readlane(pgv, grp);
-        const int key = key0 + 16 * grp;
-        const int rows = C.has(page) ? min(max(limit - key, 0), 16) : 0;
-        const int64_t off = ((rows ? page : 0) * C.page_stride + kh * C.head_stride +
-                             (key & (C.page - 1)) * C.slot_stride) * T::EB;
+        const uint64_t off =
+            ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off_l >> 32), grp) << 32) |
+            (uint32_t)__builtin_amdgcn_readlane((int)off_l, grp);
+        const uint64_t ka = k_base + off, va = v_base + off;
         u32x4 rk, rv;
-        const uint64_t ka = (uint64_t)(uintptr_t)(C.k + off), va = (uint64_t)(uintptr_t)(C.v + off);
-        rk[0] = __builtin_amdgcn_readfirstlane((uint32_t)ka);
-        rk[1] = __builtin_amdgcn_readfirstlane((uint32_t)(ka >> 32) & 0xffffu);
-        rv[0] = __builtin_amdgcn_readfirstlane((uint32_t)va);
-        rv[1] = __builtin_amdgcn_readfirstlane((uint32_t)(va >> 32) & 0xffffu);
-        rk[2] = rv[2] = __builtin_amdgcn_readfirstlane(rows * slot_bytes);
+        rk[0] = (uint32_t)ka;
+        rk[1] = (uint32_t)(ka >> 32);
+        rv[0] = (uint32_t)va;
+        rv[1] = (uint32_t)(va >> 32);
+        rk[2] = rv[2] = __builtin_amdgcn_readlane((int)size_l, grp);
         rk[3] = rv[3] = 0x00020000u;
-#pragma unroll
-        for (int q = 0; q < T::NQ; ++q) {
-          const int base = 16 * grp + (T::IPG >= 4 ? (q * 4 + w) * T::RI : (w & 1) * T::RI);
+        unroll<T::NQ>([&](auto q) {
           uint32_t hide = 0;  // positions before the window: zeros as well
           if (below) {
-            const int kk = key + l_row[q];
+            const int kk = key0 + 16 * grp + l_row[q];
             hide = kk < w_first && kk >= A.sinks ? 0x80000000u : 0u;
           }
-          dma16(rk, k_off[q] | hide, lds0 + (2 * buf) * T::BUF + base * T::RB);
-          dma16(rv, v_off[q] | hide, lds0 + (2 * buf + 1) * T::BUF + base * T::RB);
+          constexpr int at = (decltype(n)::value * (T::IPG >= 4 ? T::IPG : 4) +
+                              4 * decltype(q)::value) * 1024;
+          dma16<at>(rk, k_off[q] | hide, to);
+          dma16<at + T::BUF>(rv, v_off[q] | hide, to);
+        });
+      });
+    };
+
+    // Fragment addresses in the first buffer: step k of a K row and output tile d
+    // of V differ by an exclusive or below 256 bytes (the permutation's reach) and
+    // by a plain offset above; the buffers' parity is one more bit to flip.
+    constexpr int KX = std::min(T::QS, T::RB >= 256 ? 8 : 4);
+    constexpr int VX = T::F32 ? 1 : std::min(T::OT, 4);
+    uint32_t kx[KX], vx[VX];
+#pragma unroll
+    for (int k = 0; k < KX; ++k)
+      kx[k] = lds0 + col * T::RB + (((h ^ T::swz_k(col & 15)) * 16) ^ (k * 32));
+    if constexpr (T::F32) {
+      vx[0] = lds0 + T::BUF + 4 * h * T::RB + col * (HD == 64 ? 8 : 16);
+    } else {
+      const int vr = 4 * h + ((lane & 15) >> 2);
+#pragma unroll
+      for (int d = 0; d < VX; ++d)
+        vx[d] = lds0 + T::BUF + vr * T::RB + (lane & 3) * 8 +
+                (((((lane >> 4) & 1) * 2) ^ T::swz_v(vr) ^ (4 * d)) * 16);
+    }
+    auto read_k = [&](int f) {  // fragment f = t · QS + k
+      const int t = f / T::QS, k = f % T::QS;
+      return read16(kx[k % KX] + (k / KX) * KX * 32 + t * 32 * T::RB);
+    };
+    auto read_v = [&](int f) {  // fragment f = j · OT + d
+      const int j = f / T::OT, d = f % T::OT;
+      const uint32_t at = vx[d % VX] + (d / VX) * VX * 64 + 16 * j * T::RB;
+      const uint2 a = read_tr(at), b = read_tr(at + 8 * T::RB);
+      return uint4{a.x, a.y, b.x, b.y};
+    };
+    // One tile of the wave's rows. Fragments are read kAhead before their product
+    // and the order is pinned: left alone the compiler reads each right before
+    // its product and waits. Each step of the second product computes the weights
+    // of the next.
+    constexpr int kAhead = 4;
+    auto tile_step = [&](int key0, uint32_t bad, bool all) {
+      constexpr int KF = T::KS * T::QS;
+      f32x16 x[T::KS];
+#pragma unroll
+      for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x[t][e] = 0.f;
+      {
+        uint4 f[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < KF; ++i) {
+          const uint4 kf = f[i % kAhead], q = qf[i % T::QS];
+          f32x16& acc = x[i / T::QS];
+          if constexpr (T::F32) {
+            mma_f32(acc, __uint_as_float(kf.x), __uint_as_float(q.x));
+            mma_f32(acc, __uint_as_float(kf.y), __uint_as_float(q.y));
+            mma_f32(acc, __uint_as_float(kf.z), __uint_as_float(q.z));
+            mma_f32(acc, __uint_as_float(kf.w), __uint_as_float(q.w));
+          } else {
+            mma<DT>(acc, kf, q);
+          }
+          if (i + kAhead < KF) f[i % kAhead] = read_k(i + kAhead);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+      constexpr int VF = 2 * T::KS * T::OT;
+      uint4 vf[T::F32 ? 1 : kAhead];
+      if constexpr (!T::F32) {
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) vf[i] = read_v(i);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      if (!all) {
+#pragma unroll
+        for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int key = key0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+            const bool see = key <= p && (key >= first || key < A.sinks) &&
+                             !((bad >> (2 * t + (e >> 3))) & 1);
+            x[t][e] = see ? x[t][e] : -INFINITY;
+          }
+      }
+      // the scores as whole registers again (else the two paths meet in 16 copies
+      // a vector)
+#pragma unroll
+      for (int t = 0; t < T::KS; ++t) asm("" : "+v"(x[t]));
+      float mx = x[0][0];
+#pragma unroll
+      for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
+      mx = fmaxf(mx, __shfl_xor(mx, 32)) * A.scale_log2;
+      // o and l keep an older maximum while it is at most 2^8 too small: the
+      // weights stay in range and most tiles need no scaling
+      if (__any(mx > m + 8.f)) {
+        const float top = fmaxf(m, mx);
+        const float a = exp2f(m - (top == -INFINITY ? 0.f : top));
+        l *= a;
+#pragma unroll
+        for (int d = 0; d < T::OT; ++d)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) o[d][e] *= a;
+        m = top;
+      }
+      const float base = (m == -INFINITY ? 0.f : m) - kBias;
+      auto weight = [&](int i) {
+        const float y = __builtin_amdgcn_exp2f(fmaf(x[i >> 4][i & 15], A.scale_log2, -base));
+        x[i >> 4][i & 15] = y;
+        l += y;
+      };
+      if constexpr (T::F32) {
+#pragma unroll
+        for (int i = 0; i < 16 * T::KS; ++i) weight(i);
+#pragma unroll
+        for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const uint32_t at = vx[0] + (32 * t + 8 * (e >> 2) + (e & 3)) * T::RB;
+            if constexpr (HD == 64) {
+              const uint2 v = read8(at);
+              mma_f32(o[0], __uint_as_float(v.x), x[t][e]);
+              mma_f32(o[1], __uint_as_float(v.y), x[t][e]);
+            } else {
+#pragma unroll
+              for (int d = 0; d < T::OT; d += 4) {
+                const uint4 v = read16(at + d * 128);
+                mma_f32(o[d], __uint_as_float(v.x), x[t][e]);
+                mma_f32(o[d + 1], __uint_as_float(v.y), x[t][e]);
+                mma_f32(o[d + 2], __uint_as_float(v.z), x[t][e]);
+                mma_f32(o[d + 3], __uint_as_float(v.w), x[t][e]);
+              }
+            }
+          }
+      } else {
+        auto packed = [&](int j) {
+          const f32x16& y = x[j >> 1];
+          const int e = 8 * (j & 1);
+          return uint4{pack2<DT>(y[e], y[e + 1]), pack2<DT>(y[e + 2], y[e + 3]),
+                       pack2<DT>(y[e + 4], y[e + 5]), pack2<DT>(y[e + 6], y[e + 7])};
+        };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight(i);
+        uint4 pf = packed(0);
+#pragma unroll
+        for (int i = 0; i < VF; ++i) {
+          const int j = i / T::OT, d = i % T::OT;
+          mma<DT>(o[d], vf[i % kAhead], pf);
+          if (i + kAhead < VF) vf[i % kAhead] = read_v(i + kAhead);
+          if (j + 1 < 2 * T::KS) {
+#pragma unroll
+            for (int k = 8 * d / T::OT; k < 8 * (d + 1) / T::OT; ++k) weight(8 * (j + 1) + k);
+            if (d == T::OT - 1) pf = packed(j + 1);
+          }
+          __builtin_amdgcn_sched_barrier(0);
         }
       }
     };
-
-    // fragment addresses within a buffer
-    const uint32_t ka = col * T::RB + (h ^ T::swz_k(col & 15)) * 16;
-    uint32_t va;
-    if constexpr (T::F32)
-      va = 4 * h * T::RB + col * (HD == 64 ? 8 : 16);
-    else
-      va = (4 * h + ((lane & 15) >> 2)) * T::RB + (lane & 3) * 8 +
-           ((((lane >> 4) & 1) ^ (T::swz_v(4 * h + ((lane & 15) >> 2)) >> 1)) * 32);
 
     const int rounds = (hi - lo + T::TEAMS - 1) / T::TEAMS;
     int32_t pgv = 0;
@@ -278,107 +446,19 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
         load_tile(i + T::TEAMS, (n + 1) & 1, pgv);
         pgv = pages_of(i + 2 * T::TEAMS);
       }
+      if (n > 0) {  // the other buffers
+#pragma unroll
+        for (int k = 0; k < KX; ++k) kx[k] ^= 2 * T::BUF;
+#pragma unroll
+        for (int k = 0; k < VX; ++k) vx[k] ^= 2 * T::BUF;
+      }
       if (i >= hi || !any) continue;
       const int key0 = range.tile(i) * T::KT;
       // nothing of it is seen by the wave
       if (key0 > wp_max || (key0 + T::KT <= wfirst_min && key0 >= A.sinks)) continue;
-      const uint32_t kb = lds0 + 2 * (n & 1) * T::BUF, vb = kb + T::BUF;
-
-      f32x16 x[T::KS];
-#pragma unroll
-      for (int t = 0; t < T::KS; ++t) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = 0.f;
-#pragma unroll
-        for (int k = 0; k < T::QS; ++k) {
-          const uint4 kf = read16(kb + (ka ^ (k * 32)) + t * 32 * T::RB);
-          if constexpr (T::F32) {
-            mma_f32(x[t], __uint_as_float(kf.x), __uint_as_float(qf[k].x));
-            mma_f32(x[t], __uint_as_float(kf.y), __uint_as_float(qf[k].y));
-            mma_f32(x[t], __uint_as_float(kf.z), __uint_as_float(qf[k].z));
-            mma_f32(x[t], __uint_as_float(kf.w), __uint_as_float(qf[k].w));
-          } else {
-            mma<DT>(x[t], kf, qf[k]);
-          }
-        }
-      }
       const bool all = key0 + T::KT - 1 <= wp_min && !bad &&
                        (key0 >= wfirst_max || key0 + T::KT <= A.sinks);
-      if (!all) {
-#pragma unroll
-        for (int t = 0; t < T::KS; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = key0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-            const bool see = key <= p && (key >= first || key < A.sinks) &&
-                             !((bad >> (2 * t + (e >> 3))) & 1);
-            x[t][e] = see ? x[t][e] : -INFINITY;
-          }
-      }
-      float mx = x[0][0];
-#pragma unroll
-      for (int t = 0; t < T::KS; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32)) * A.scale_log2;
-      // o and l keep an older maximum while it is at most 2^8 too small: the
-      // weights stay in range and most tiles need no scaling
-      if (__any(mx > m + 8.f)) {
-        const float top = fmaxf(m, mx);
-        const float a = exp2f(m - (top == -INFINITY ? 0.f : top));
-        l *= a;
-#pragma unroll
-        for (int d = 0; d < T::OT; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[d][e] *= a;
-        m = top;
-      }
-      const float base = (m == -INFINITY ? 0.f : m) - kBias;
-      float sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < T::KS; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          x[t][e] = __builtin_amdgcn_exp2f(fmaf(x[t][e], A.scale_log2, -base));
-          sum += x[t][e];
-        }
-      l += sum;
-      if constexpr (T::F32) {
-#pragma unroll
-        for (int t = 0; t < T::KS; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t at = vb + va + (32 * t + 8 * (e >> 2) + (e & 3)) * T::RB;
-            if constexpr (HD == 64) {
-              const uint2 v = read8(at);
-              mma_f32(o[0], __uint_as_float(v.x), x[t][e]);
-              mma_f32(o[1], __uint_as_float(v.y), x[t][e]);
-            } else {
-#pragma unroll
-              for (int d = 0; d < T::OT; d += 4) {
-                const uint4 v = read16(at + d * 128);
-                mma_f32(o[d], __uint_as_float(v.x), x[t][e]);
-                mma_f32(o[d + 1], __uint_as_float(v.y), x[t][e]);
-                mma_f32(o[d + 2], __uint_as_float(v.z), x[t][e]);
-                mma_f32(o[d + 3], __uint_as_float(v.w), x[t][e]);
-              }
-            }
-          }
-      } else {
-#pragma unroll
-        for (int j = 0; j < 2 * T::KS; ++j) {
-          const int e = 8 * (j & 1);
-          const f32x16& y = x[j >> 1];
-          const uint4 pf = {pack2<DT>(y[e], y[e + 1]), pack2<DT>(y[e + 2], y[e + 3]),
-                            pack2<DT>(y[e + 4], y[e + 5]), pack2<DT>(y[e + 6], y[e + 7])};
-#pragma unroll
-          for (int d = 0; d < T::OT; ++d) {
-            const uint32_t at = vb + (va ^ (d * 64)) + 16 * j * T::RB;
-            const uint2 a = read_tr(at), b = read_tr(at + 8 * T::RB);
-            mma<DT>(o[d], uint4{a.x, a.y, b.x, b.y}, pf);
-          }
-        }
-      }
+      tile_step(key0, bad, all);
     }
     l += __shfl_xor(l, 32);
 
