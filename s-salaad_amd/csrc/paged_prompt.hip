@@ -105,6 +105,15 @@ __device__ __forceinline__ void mma_f32(f32x16& acc, float a, float b) {
   acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, acc, 0, 0, 0);
 }
 
+// Where paths meet, keeps accumulators in the registers the matrix instructions
+// use. (Else each path leaves its elements in registers of its own, which are
+// copied, 16 a vector, and held twice.)
+template <int N>
+__device__ __forceinline__ void whole_registers(f32x16 (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm("" : "+v"(v[i]));
+}
+
 template <typename F, int... I>
 __device__ __forceinline__ void unroll_over(F& f, std::integer_sequence<int, I...>) {
   (f(std::integral_constant<int, I>{}), ...);
@@ -227,45 +236,47 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
       const int key = range.tile(min(i, hi - 1)) * T::KT + 16 * (lane % (T::KT / 16));
       return table[min(key >> C.log2_page, C.cols - 1)];
     };
-    // Each lane settles one group of 16 positions (group lane % (KT / 16)): its
-    // place in the pools and the bytes of it that are loaded; the loads then read
-    // theirs from that lane.
-    auto load_tile = [&](int i, int buf, int32_t page) {
-      constexpr int KG = T::KT / 16;
+    // The next tile's loads. Each lane settles one group of 16 positions (group
+    // lane % (KT / 16)): its place in the pools and the bytes of it that are
+    // loaded; load<I> reads them from that lane and issues the wave's I-th loads of
+    // K and V. A tile that does not exist loads zeros.
+    constexpr int KG = T::KT / 16;
+    constexpr int LOADS = (T::IPG >= 4 ? KG : KG / 2) * T::NQ;
+    uint64_t off_l = 0;
+    uint32_t size_l = 0, next_lds = 0, hide_span = 0;
+    int hide_from = 0;
+    auto next_tile = [&](int i, int buf, int32_t page) {
       const int key0 = range.tile(i) * T::KT;
       const int key_l = key0 + 16 * (lane % KG);
-      const bool has = C.has(page);
-      const uint64_t off_l = (uint64_t)(uint32_t)(has ? page : 0) * page_bytes +
-                             (uint32_t)(key_l & (C.page - 1)) * slot_bytes;
-      const uint32_t size_l = has ? min(max(limit - key_l, 0), 16) * slot_bytes : 0u;
-      const bool below = key0 < w_first && key0 + T::KT > A.sinks;
-      // instruction (n, q) fills 1 KiB at n · max(IPG, 4) + 4 q + w
-      const uint32_t to = lds0 + 2 * buf * T::BUF + w * 1024;
-      unroll<(T::IPG >= 4 ? KG : KG / 2)>([&](auto n) {
-        const int grp = T::IPG >= 4 ? n : 2 * n + (w >> 1);
-        const uint64_t off =
-            ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off_l >> 32), grp) << 32) |
-            (uint32_t)__builtin_amdgcn_readlane((int)off_l, grp);
-        const uint64_t ka = k_base + off, va = v_base + off;
-        u32x4 rk, rv;
-        rk[0] = (uint32_t)ka;
-        rk[1] = (uint32_t)(ka >> 32);
-        rv[0] = (uint32_t)va;
-        rv[1] = (uint32_t)(va >> 32);
-        rk[2] = rv[2] = __builtin_amdgcn_readlane((int)size_l, grp);
-        rk[3] = rv[3] = 0x00020000u;
-        unroll<T::NQ>([&](auto q) {
-          uint32_t hide = 0;  // positions before the window: zeros as well
-          if (below) {
-            const int kk = key0 + 16 * grp + l_row[q];
-            hide = kk < w_first && kk >= A.sinks ? 0x80000000u : 0u;
-          }
-          constexpr int at = (decltype(n)::value * (T::IPG >= 4 ? T::IPG : 4) +
-                              4 * decltype(q)::value) * 1024;
-          dma16<at>(rk, k_off[q] | hide, to);
-          dma16<at + T::BUF>(rv, v_off[q] | hide, to);
-        });
-      });
+      const bool has = C.has(page) && i < hi;
+      off_l = (uint64_t)(uint32_t)(has ? page : 0) * page_bytes +
+              (uint32_t)(key_l & (C.page - 1)) * slot_bytes;
+      size_l = has ? min(max(limit - key_l, 0), 16) * slot_bytes : 0u;
+      next_lds = lds0 + 2 * buf * T::BUF + w * 1024;
+      // positions from sinks to the window's first: zeros as well
+      hide_from = key0 - A.sinks;
+      hide_span = key0 < w_first ? max(w_first - A.sinks, 0) : 0;
+    };
+    auto load = [&](auto at) {
+      constexpr int n = decltype(at)::value / T::NQ, q = decltype(at)::value % T::NQ;
+      const int grp = T::IPG >= 4 ? n : 2 * n + (w >> 1);
+      const uint64_t off =
+          ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off_l >> 32), grp) << 32) |
+          (uint32_t)__builtin_amdgcn_readlane((int)off_l, grp);
+      const uint64_t ka = k_base + off, va = v_base + off;
+      u32x4 rk, rv;
+      rk[0] = (uint32_t)ka;
+      rk[1] = (uint32_t)(ka >> 32);
+      rv[0] = (uint32_t)va;
+      rv[1] = (uint32_t)(va >> 32);
+      rk[2] = rv[2] = __builtin_amdgcn_readlane((int)size_l, grp);
+      rk[3] = rv[3] = 0x00020000u;
+      const uint32_t hide =
+          (uint32_t)(hide_from + 16 * grp + l_row[q]) < hide_span ? 0x80000000u : 0u;
+      // the instruction fills 1 KiB at n · max(IPG, 4) + 4 q + w
+      constexpr int to = (n * (T::IPG >= 4 ? T::IPG : 4) + 4 * q) * 1024;
+      dma16<to>(rk, k_off[q] | hide, next_lds);
+      dma16<to + T::BUF>(rv, v_off[q] | hide, next_lds);
     };
 
     // Fragment addresses in the first buffer: step k of a K row and output tile d
@@ -313,8 +324,8 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
 #pragma unroll
         for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
         __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < KF; ++i) {
+        unroll<KF>([&](auto at) {
+          constexpr int i = decltype(at)::value;
           const uint4 kf = f[i % kAhead], q = qf[i % T::QS];
           f32x16& acc = x[i / T::QS];
           if constexpr (T::F32) {
@@ -325,9 +336,11 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
           } else {
             mma<DT>(acc, kf, q);
           }
-          if (i + kAhead < KF) f[i % kAhead] = read_k(i + kAhead);
+          if constexpr (i + kAhead < KF) f[i % kAhead] = read_k(i + kAhead);
+          if constexpr (i % (KF / LOADS) == 1)
+            load(std::integral_constant<int, i / (KF / LOADS)>{});
           __builtin_amdgcn_sched_barrier(0);
-        }
+        });
       }
       constexpr int VF = 2 * T::KS * T::OT;
       uint4 vf[T::F32 ? 1 : kAhead];
@@ -347,16 +360,17 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
             x[t][e] = see ? x[t][e] : -INFINITY;
           }
       }
-      // the scores as whole registers again (else the two paths meet in 16 copies
-      // a vector)
-#pragma unroll
-      for (int t = 0; t < T::KS; ++t) asm("" : "+v"(x[t]));
+      whole_registers(x);
       float mx = x[0][0];
 #pragma unroll
       for (int t = 0; t < T::KS; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
-      mx = fmaxf(mx, __shfl_xor(mx, 32)) * A.scale_log2;
+      {  // with the row's other lane
+        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
+                                                           false, false);
+        mx = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * A.scale_log2;
+      }
       // o and l keep an older maximum while it is at most 2^8 too small: the
       // weights stay in range and most tiles need no scaling
       if (__any(mx > m + 8.f)) {
@@ -425,41 +439,49 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
 
     const int rounds = (hi - lo + T::TEAMS - 1) / T::TEAMS;
     int32_t pgv = 0;
-    uint32_t bad = 0, bad_next = 0;  // groups of 16 of the tile that lie on no page
+    uint32_t bad_next = 0;  // groups of 16 of the tile that lie on no page
     auto missing = [&](int32_t pg) {
       return (uint32_t)__ballot(!C.has(pg)) & ((1u << (T::KT / 16)) - 1);
     };
     barrier();  // the rows before have left the buffers
-    if (lo + team < hi) {
+    if (rounds > 0) {
       pgv = pages_of(lo + team);
       bad_next = missing(pgv);
-      load_tile(lo + team, 0, pgv);
+      next_tile(lo + team, 0, pgv);
+      unroll<LOADS>(load);
+      pgv = pages_of(lo + team + T::TEAMS);
     }
-    pgv = lo + team + T::TEAMS < hi ? pages_of(lo + team + T::TEAMS) : 0;
-    for (int n = 0; n < rounds; ++n) {
-      const int i = lo + n * T::TEAMS + team;
-      wait_loads();
-      barrier();
-      bad = bad_next;
-      if (i + T::TEAMS < hi) {
-        bad_next = missing(pgv);
-        load_tile(i + T::TEAMS, (n + 1) & 1, pgv);
+    if (!any) {  // a wave without rows only loads
+      for (int n = 0; n < rounds; ++n) {
+        const int i = lo + n * T::TEAMS + team;
+        wait_loads();
+        barrier();
+        next_tile(i + T::TEAMS, (n + 1) & 1, pgv);
         pgv = pages_of(i + 2 * T::TEAMS);
+        unroll<LOADS>(load);
       }
-      if (n > 0) {  // the other buffers
+    } else {
+      for (int n = 0; n < rounds; ++n) {
+        const int i = lo + n * T::TEAMS + team;
+        wait_loads();
+        barrier();
+        // a tile past the end, or seen by no row, runs masked: its workgroup waits
+        // for the others' anyway, and a path around it costs copies of o
+        const uint32_t bad = i < hi ? bad_next : ~0u;
+        bad_next = missing(pgv);
+        next_tile(i + T::TEAMS, (n + 1) & 1, pgv);
+        pgv = pages_of(i + 2 * T::TEAMS);
+        const int key0 = range.tile(i) * T::KT;
+        const bool all = key0 + T::KT - 1 <= wp_min && !bad &&
+                         (key0 >= wfirst_max || key0 + T::KT <= A.sinks);
+        tile_step(key0, bad, all);
 #pragma unroll
-        for (int k = 0; k < KX; ++k) kx[k] ^= 2 * T::BUF;
+        for (int k = 0; k < KX; ++k) kx[k] ^= 2 * T::BUF;  // the other buffers
 #pragma unroll
         for (int k = 0; k < VX; ++k) vx[k] ^= 2 * T::BUF;
       }
-      if (i >= hi || !any) continue;
-      const int key0 = range.tile(i) * T::KT;
-      // nothing of it is seen by the wave
-      if (key0 > wp_max || (key0 + T::KT <= wfirst_min && key0 >= A.sinks)) continue;
-      const bool all = key0 + T::KT - 1 <= wp_min && !bad &&
-                       (key0 >= wfirst_max || key0 + T::KT <= A.sinks);
-      tile_step(key0, bad, all);
     }
+    wait_loads();
     l += __shfl_xor(l, 32);
 
     // the second team's part joins the first's
