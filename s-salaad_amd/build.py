@@ -12,6 +12,8 @@ read from plans and records and report a bad one in the call's status word
 
 The host call path csrc_py/hostcall.c is built with the C compiler into
 `ssalaad_amd/hostcall.<abi>.so`, a CPython extension that links to neither.
+csrc_py/tensorcall.cpp, the paged operators' call path, is one over torch's C++
+tensors: `ssalaad_amd/tensorcall.<abi>.so`, for the torch that builds it.
 
 Usage: python s-salaad_amd/build.py [-v] [--checked]
 """
@@ -98,8 +100,34 @@ def build_hostcall(verbose: bool = False) -> Path:
     return out
 
 
+def build_tensorcall(verbose: bool = False) -> Path:
+    import torch
+
+    cxx = shutil.which("g++") or shutil.which("c++") or shutil.which("clang++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler found; the tensor call path cannot be built")
+    root = Path(torch.__file__).parent
+    out = HERE / "ssalaad_amd" / ("tensorcall" + sysconfig.get_config_var("EXT_SUFFIX"))
+    tmp = out.with_name(out.name + ".tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-Wno-unused-function",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(HERE.parent / "include"), "-isystem", str(root / "include"),
+           "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-I", sysconfig.get_paths()["include"], str(HERE / "csrc_py" / "tensorcall.cpp"),
+           "-o", str(tmp), f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"building the tensor call path failed:\n{res.stderr}")
+    os.replace(tmp, out)
+    if verbose:
+        print(f"[build] wrote {out}")
+    return out
+
+
 def build(verbose: bool = False, jobs: int = 8, checked: bool = False) -> Path:
     build_hostcall(verbose)
+    build_tensorcall(verbose)
     hipcc = _hipcc()
     out = OUT_CHECKED if checked else OUT
     build_dir = BUILD_DIR / "checked" if checked else BUILD_DIR

@@ -256,6 +256,36 @@ def hostcall(required: bool = True):
     return _hostcall
 
 
+_tensorcall = None
+
+
+def tensorcall():
+    """The compiled call path of the paged operators, bound to the library
+    (once); raises if it was not built. Its functions return None for a call
+    they leave to Python."""
+    global _tensorcall
+    if _tensorcall is None:
+        try:
+            from . import tensorcall as mod
+        except ImportError as e:
+            raise RuntimeError(
+                "the tensor call path is not built; run `python s-salaad_amd/build.py` "
+                "(or __graft_entry__.build()) first") from e
+        mod.bind(torch._C._cuda_getCurrentRawStream, *map(entry_address, (
+            "ssl_paged_append", "ssl_paged_attention_workspace_size", "ssl_paged_attention",
+            "ssl_pages_free", "ssl_pages_fork_workspace_size", "ssl_pages_fork",
+            "ssl_pages_compact_workspace_size", "ssl_pages_compact", "ssl_token_logprobs")))
+        _tensorcall = mod
+    return _tensorcall
+
+
+def completed(out, what: str):
+    """What a tensorcall function returned, or the exception of its status."""
+    if type(out) is int:
+        check(out, what)
+    return out
+
+
 _ADDRESS: dict[str, int] = {}
 
 

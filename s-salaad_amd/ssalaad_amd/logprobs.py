@@ -32,6 +32,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     [0, vocab) scores NaN, as does every value of a row that holds a NaN, a +inf
     or nothing above -inf. Runs on torch's current stream; nothing synchronises.
     """
+    out = _lib.tensorcall().logprobs(logits, tokens, top)
+    if out is not None:
+        return TokenLogprobs(*_lib.completed(out, "ssl_token_logprobs"))
     if not logits.is_cuda:
         raise ValueError("token_logprobs runs on a ROCm GPU device; move the logits there first")
     if logits.dim() != 2 or logits.shape[1] == 0:

@@ -17,7 +17,12 @@ float32, bfloat16 and float16; head_dim 64, 128 or 256; pages of 16 to 1024
 positions (a power of two); any number of query heads per key/value head. Every
 call runs on torch's current stream, reads lengths, positions and page numbers
 on the device (none synchronises) and may be captured into a HIP graph. Page
-numbers outside the pool are treated as no page. There is no CPU path.
+numbers outside the pool are treated as no page. There is no CPU path and no
+gradient.
+
+Each function first hands its call to the compiled path (csrc_py/tensorcall.cpp),
+which takes arguments that are as the kernels want them; what it leaves is
+checked, and laid out anew where needed, here.
 """
 
 from __future__ import annotations
@@ -138,6 +143,10 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
     position without an angle gives a zero row; it and one without a page are
     not written. No two tokens may share a place.
     """
+    out = _lib.tensorcall().append(q, k, v, cos, sin, k_pool, v_pool, table, seqs, positions,
+                                   q_norm, k_norm, eps)
+    if out is not None:
+        return _lib.completed(out, "ssl_paged_append")
     pools = _pools(k_pool, v_pool, False)
     dev, hd, kv = k_pool.device, pools[10], pools[8]
     if q.dim() != 3:
@@ -182,6 +191,10 @@ def paged_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: torch.T
 
 
 def _attention(q, k_pool, v_pool, table, lengths, cu, window, sinks, scale, max_tokens, max_length):
+    out = _lib.tensorcall().attention(q, k_pool, v_pool, table, lengths, cu, window, sinks, scale,
+                                      max_tokens, max_length)
+    if out is not None:
+        return _lib.completed(out, "ssl_paged_attention")
     pools = _pools(k_pool, v_pool, False)
     dev, hd = k_pool.device, pools[10]
     if q.dim() != 3:
@@ -272,6 +285,9 @@ def free_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
     [pages] int32 counts the entries that name a page; one at 0 is free. A
     sequence named twice ends once; one out of range is passed over. The given
     tensors stay as they are."""
+    out = _lib.tensorcall().free(table, lengths, refs, seqs)
+    if out is not None:
+        return _lib.completed(out, "ssl_pages_free")
     dev = _on_gpu(table, "the page table")
     if seqs.dim() != 1:
         raise ValueError("seqs must be 1-D")
@@ -296,6 +312,9 @@ def fork_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
     [n] bool is False, and nothing changes, where src or dst is out of range,
     dst is not empty or was named before, a page of src is missing, or no page
     is free."""
+    out = _lib.tensorcall().fork(table, lengths, refs, k_pool, v_pool, src, dst)
+    if out is not None:
+        return _lib.completed(out, "ssl_pages_fork")
     pools = _pools(k_pool, v_pool, True)
     dev = k_pool.device
     if src.dim() != 1:
@@ -324,6 +343,9 @@ def compact_pages(table: torch.Tensor, refs: torch.Tensor, k_pool: torch.Tensor,
     `live` (0-d int32) of them, the i-th used page at or above it moves into the
     i-th free one below it, in every layer (in place in the pools), and the
     table's entries follow. Pages from `live` on are free afterwards."""
+    out = _lib.tensorcall().compact(table, refs, k_pool, v_pool)
+    if out is not None:
+        return _lib.completed(out, "ssl_pages_compact")
     pools = _pools(k_pool, v_pool, True)
     dev = k_pool.device
     table, refs, table_out, refs_out = _state(table, refs, dev)

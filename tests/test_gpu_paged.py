@@ -602,3 +602,68 @@ def test_a_captured_step_replays(gpu_device):
         for a, b in zip(eager, want):
             assert torch.equal(a, b), i
         q.add_(0)  # eager work between the replays
+
+
+# ------------------------------------------------------------- call paths --
+class _Nothing:
+    """A compiled path that takes no call."""
+
+    def __getattr__(self, name):
+        return lambda *a: None
+
+
+def test_the_compiled_and_the_python_path_issue_the_same_calls(gpu_device, monkeypatch):
+    import ssalaad_amd as sa
+    from ssalaad_amd import _lib
+
+    dev = gpu_device
+
+    def results():
+        g = torch.Generator().manual_seed(12)
+        lens, counts = [40, 17, 0], [9, 17, 0]
+        table, pages = pc.pages_of(lens, 16, g, cols=4)
+        kp, vp = (t.to(dev) for t in pc.cache(pages, 2, 16, 64, torch.bfloat16, g))
+        q, k, v = (torch.randn(26, h, 64, generator=g).to(torch.bfloat16).to(dev) for h in (4, 2, 2))
+        cos, sin = (t.to(dev) for t in pc.angles(64, 64))
+        w = (1 + torch.randn(64, generator=g)).to(torch.bfloat16).to(dev)
+        owners, pos = pc.chunk_rows(counts, lens)
+        i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+        tb, L = table.to(dev), i32(*lens)
+        refs = torch.zeros(pages, dtype=torch.int32)
+        refs[table[table >= 0].long()] = 1
+        out = [sa.paged_append(q, k, v, cos, sin, kp, vp, tb, i32(*owners), i32(*pos), q_norm=w)]
+        out.append(sa.paged_decode_attention(q[:3], kp, vp, tb, L, window=20, sinks=2, scale=0.2))
+        out.append(sa.paged_prompt_attention(q, kp, vp, tb, L, i32(0, 9, 26, 26), max_tokens=17,
+                                             max_length=40))
+        out += sa.fork_pages(tb, L, refs.to(dev), kp, vp, i32(0), i32(2))
+        out += sa.free_pages(*out[-4:-1], i32(1))
+        out += sa.compact_pages(out[-3], out[-1], kp, vp)
+        out += sa.token_logprobs(torch.randn(4, 99, generator=g).to(dev),
+                                 torch.arange(4, device=dev), top=5)
+        return [t.cpu() for t in (*out, kp, vp)]
+
+    taken = results()
+    monkeypatch.setattr(_lib, "tensorcall", _Nothing)
+    for a, b in zip(taken, results(), strict=True):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_the_compiled_path_takes_what_a_step_passes(gpu_device):
+    from ssalaad_amd import _lib
+
+    tc, dev = _lib.tensorcall(), gpu_device
+    z = lambda *s, dtype=torch.bfloat16: torch.zeros(*s, dtype=dtype, device=dev)  # noqa: E731
+    i = lambda *s: z(*s, dtype=torch.int32)  # noqa: E731
+    pool = z(9, 2, 16, 64)
+    args = [z(3, 2, 64), pool, pool, i(3, 5), i(3), None, 0, 0, None, 1, None]
+    assert torch.is_tensor(tc.attention(*args))
+    assert torch.is_tensor(tc.attention(torch.nn.Parameter(args[0]), *args[1:]))
+    for k, bad in ((0, z(3, 2, 128)[:, :, ::2]), (0, z(3, 3, 64)), (0, args[0].float()),
+                   (1, z(9, 2, 17, 64)[:, :, 1:]), (3, i(3, 5).long()), (4, i(6)[::2]),
+                   (6, -1), (7, 1.5), (8, "x"), (10, -1)):
+        assert tc.attention(*args[:k], bad, *args[k + 1:]) is None, k
+    big = z(9, 2, 16, 64, dtype=torch.int8)
+    assert tc.attention(z(3, 2, 64, dtype=torch.int8), big, big, *args[3:]) is None
+    # a page size without a kernel is the C ABI's refusal
+    odd = z(9, 2, 24, 64)
+    assert tc.attention(args[0], odd, odd, *args[3:]) == _lib.SSL_ERR_UNSUPPORTED

@@ -217,3 +217,34 @@ def test_there_is_no_cpu_path():
 def test_struct_sizes_are_whole_words():
     for st in (paged._APPEND, paged._ATTENTION, paged._PAGES, logprobs._ARGS):
         assert isinstance(st, struct.Struct) and st.size % 8 == 0
+
+
+# ------------------------------------------------------ the compiled path --
+def test_the_compiled_path_leaves_cpu_tensors_to_python():
+    """None for every function: nothing is launched, the Python checks decide."""
+    tc = _lib.tensorcall()
+    pool = _t(9, 2, 16, 64)
+    assert tc.append(*[_t(1, 2, 64)] * 3, _t(9, 32), _t(9, 32), pool, pool, _i(1, 4), _i(1), _i(1),
+                     None, None, 1e-6) is None
+    assert tc.attention(_t(3, 2, 64), pool, pool, _i(3, 5), _i(3), None, 0, 0, None, 1, None) is None
+    assert tc.free(_i(3, 5), _i(3), _i(9), _i(1)) is None
+    assert tc.fork(_i(3, 5), _i(3), _i(9), pool, pool, _i(1), _i(1)) is None
+    assert tc.compact(_i(3, 5), _i(9), pool, pool) is None
+    assert tc.logprobs(torch.zeros(2, 9), torch.zeros(2, dtype=torch.int64), 1) is None
+    for fn in (tc.append, tc.attention, tc.free, tc.fork, tc.compact, tc.logprobs):
+        assert fn() is None and fn(None) is None and fn(*[object()] * 7) is None
+    with pytest.raises(TypeError):
+        tc.bind(None)
+    with pytest.raises(ValueError):
+        tc.bind(None, *[0] * 9)
+
+
+def test_a_status_becomes_the_exception_of_the_c_abi():
+    with pytest.raises(ValueError):
+        _lib.completed(_lib.SSL_ERR_INVALID, "call")
+    with pytest.raises(TypeError):
+        _lib.completed(_lib.SSL_ERR_UNSUPPORTED, "call")
+    with pytest.raises(RuntimeError):
+        _lib.completed(_lib.SSL_ERR_HIP, "call")
+    t = torch.zeros(1)
+    assert _lib.completed(t, "call") is t
