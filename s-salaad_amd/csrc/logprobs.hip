@@ -3,9 +3,11 @@
 //   d_i = x_i − max x,  S = Σ exp(d_i),  T = Σ exp(d_i)·d_i
 //   logprob = d_token − log S,  entropy = log S − T / S
 // One pass over the row: each thread keeps a running maximum of its elements
-// and S and T relative to it. S is summed in 64 bits, so that a row with one
-// likely token keeps the digits of log S near zero; a vector's terms of T, where
-// the maximum itself adds nothing, are summed in fp32 and then in 64 bits.
+// and S and T relative to it, scaled (without a branch: some lane of a wave meets
+// a new maximum in almost every group) once a group of vectors. S is summed in
+// 64 bits, so that a row with one likely token keeps the digits of log S near
+// zero; a group's terms of T, where the maximum itself adds nothing, are summed
+// in fp32 and then in 64 bits.
 //
 // The alternatives are ordered by a 64-bit key, the logit's bits in an
 // order-preserving form over the inverted index: larger logits first, equal ones
@@ -15,6 +17,8 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+
+#include <type_traits>
 
 #include "abi_internal.h"
 #include "slr_common.h"
@@ -48,23 +52,65 @@ __device__ __forceinline__ float logit_of(uint64_t key) {
 }
 __device__ __forceinline__ int index_of(uint64_t key) { return (int)(0xffffffffu - (uint32_t)key); }
 
-// f over the workgroup's values, in a fixed order
-template <int NT, typename T, typename F>
-__device__ __forceinline__ T reduce(T v, F f) {
-  __shared__ T part[NT / 64];
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) v = f(v, __shfl_xor(v, o));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = part[0];
-#pragma unroll
-  for (int w = 1; w < NT / 64; ++w) v = f(v, part[w]);
-  return v;
+// The value of lane (l ^ O), for a wave's exchanges without LDS: quads, then
+// mirrored halves and rows (l ^ 4 = l ^ 7 ^ 3, l ^ 8 = l ^ 15 ^ 7), then swaps of
+// rows and halves.
+template <int O>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+  constexpr int kQuadRev = 0x1b, kHalfMirror = 0x141, kMirror = 0x140;
+  const auto dpp = [](uint32_t x, auto ctrl) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xf, 0xf, true);
+  };
+  if constexpr (O == 1) return dpp(v, std::integral_constant<int, 0xb1>{});
+  else if constexpr (O == 2) return dpp(v, std::integral_constant<int, 0x4e>{});
+  else if constexpr (O == 4)
+    return dpp(dpp(v, std::integral_constant<int, kHalfMirror>{}),
+               std::integral_constant<int, kQuadRev>{});
+  else if constexpr (O == 8)
+    return dpp(dpp(v, std::integral_constant<int, kMirror>{}),
+               std::integral_constant<int, kHalfMirror>{});
+  else if constexpr (O == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int O, typename T>
+__device__ __forceinline__ T lane_xor(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, lane_xor<O>(__builtin_bit_cast(uint32_t, v)));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(T, ((uint64_t)lane_xor<O>((uint32_t)(u >> 32)) << 32) |
+                                     lane_xor<O>((uint32_t)u));
+  }
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int o) {
-  return ((uint64_t)__shfl_xor((uint32_t)(v >> 32), o) << 32) | __shfl_xor((uint32_t)v, o);
+// f over the wave's values, in a fixed order
+template <typename T, typename F>
+__device__ __forceinline__ T wave_reduce(T v, F f) {
+  v = f(v, lane_xor<1>(v));
+  v = f(v, lane_xor<2>(v));
+  v = f(v, lane_xor<4>(v));
+  v = f(v, lane_xor<8>(v));
+  v = f(v, lane_xor<16>(v));
+  return f(v, lane_xor<32>(v));
+}
+
+// One step of a descending bitonic sort over a wave.
+template <int SIZE, int O>
+__device__ __forceinline__ void sort_step(uint64_t& k, int lane) {
+  const uint64_t other = lane_xor<O>(k);
+  const bool greater = ((lane & O) == 0) == ((lane & SIZE) == 0);
+  k = (k > other) == greater ? k : other;
+}
+template <int SIZE, int O = SIZE / 2>
+__device__ __forceinline__ void sort_wave(uint64_t& k, int lane) {
+  if constexpr (SIZE > 2 && O == SIZE / 2) sort_wave<SIZE / 2>(k, lane);
+  sort_step<SIZE, O>(k, lane);
+  if constexpr (O > 1) sort_wave<SIZE, O / 2>(k, lane);
 }
 
 constexpr int kCandidates = 2048;
@@ -99,34 +145,30 @@ struct Row {
   __device__ __forceinline__ float at(int i) const { return load_scalar<DT>(x, i); }
 };
 
-// A thread's running maximum (and its first index), S and T.
+// A thread's running maximum (and the first element that holds it), S and T. The
+// maximum starts at the lowest finite value, below which only −inf lies (whose
+// weight is 0 against it).
 struct Running {
-  float m = -INFINITY;
+  float m = -3.402823466e38f;
   int first = -1;
   double S = 0, T = 0;
-  template <int N>
-  __device__ __forceinline__ void add(const float* x, int i0) {
+  // N elements; index(e) is that of the e-th, ascending
+  template <int N, typename F>
+  __device__ __forceinline__ void add(const float* x, F index) {
     float top = x[0];
 #pragma unroll
     for (int e = 1; e < N; ++e) top = fmaxf(top, x[e]);
-    if (!(top <= m)) {  // greater, or NaN throughout
-      const float shift = m - top;  // −inf at the first
-      if (S != 0) {
-        const double f = expf(shift);
-        T = f * (T + S * shift);
-        S *= f;
-      }
-      m = top;
+    int at = 0;
 #pragma unroll
-      for (int e = N - 1; e >= 0; --e)
-        if (x[e] == top) first = i0 + e;
-    }
-    if (m == -INFINITY) {
-#pragma unroll
-      for (int e = 0; e < N; ++e)
-        if (x[e] != x[e]) S = NAN;
-      return;
-    }
+    for (int e = N - 1; e > 0; --e) at = x[e] == top ? e : at;
+    at = x[0] == top ? 0 : at;
+    if (top > m || (S == 0 && top == m)) first = index(at);
+    // finite, so that an S of 0 adds 0
+    const float shift = fmaxf(m - fmaxf(m, top), -3.402823466e38f);
+    const double f = __builtin_amdgcn_exp2f(shift * 1.44269504f);
+    T = f * fma(S, (double)shift, T);
+    S *= f;
+    m = fmaxf(m, top);
     float t = 0;
 #pragma unroll
     for (int e = 0; e < N; ++e) {
@@ -139,115 +181,142 @@ struct Running {
   }
 };
 
+// The 64 largest keys of the workgroup's waves (k: each wave's, descending over
+// its lanes), descending in lists[0 .. 64). Two lists' largest are the larger of
+// one and the other reversed, a bitonic sequence.
+template <int NW>
+__device__ __forceinline__ void merge_waves(uint64_t k, uint64_t* lists, int wave, int lane) {
+  lists[wave * 64 + lane] = k;
+#pragma unroll
+  for (int n = NW / 2; n > 0; n >>= 1) {
+    __syncthreads();
+    if (wave < n) {
+      const uint64_t other = lists[(wave + n) * 64 + 63 - lane];
+      k = k > other ? k : other;
+      sort_step<64, 32>(k, lane);
+      sort_step<64, 16>(k, lane);
+      sort_step<64, 8>(k, lane);
+      sort_step<64, 4>(k, lane);
+      sort_step<64, 2>(k, lane);
+      sort_step<64, 1>(k, lane);
+      lists[wave * 64 + lane] = k;
+    }
+  }
+  __syncthreads();
+}
+
 template <int DT, int NT>
 __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs A) {
   constexpr int VE = Row<DT>::VE, NW = NT / 64;
   const Row<DT> R(A);
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t tok = A.tokens[blockIdx.x];
+  const bool in = tok >= 0 && tok < A.vocab;
+  const float x_tok = R.at(in ? (int)tok : 0);  // early, beside the row
+  constexpr int U = 16 / VE * 2;  // vectors of a group: 32 elements, loaded together
   Running own;
-  // a thread of nothing above −inf has its first element for its best
-  own.first = tid < R.peel ? tid
-              : tid < R.vecs ? R.peel + tid * VE
-              : tid < R.tail ? A.vocab - R.tail + tid : -1;
   if (tid < R.peel) {
     const float x = R.at(tid);
-    own.add<1>(&x, tid);
+    own.add<1>(&x, [&](int) { return tid; });
   }
-  constexpr int U = 4;  // vectors in flight
   int v = tid;
+  const auto index = [&](int e) { return R.peel + (v + e / VE * NT) * VE + e % VE; };
   for (; v + (U - 1) * NT < R.vecs; v += U * NT) {
-    float x[U][VE];
+    float x[U * VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) R.vec(x[u], v + u * NT);
-#pragma unroll
-    for (int u = 0; u < U; ++u) own.add<VE>(x[u], R.peel + (v + u * NT) * VE);
+    for (int u = 0; u < U; ++u) R.vec(x + u * VE, v + u * NT);
+    own.add<U * VE>(x, index);
   }
-  for (; v < R.vecs; v += NT) {
-    float x[VE];
-    R.vec(x, v);
-    own.add<VE>(x, R.peel + v * VE);
+  if (v < R.vecs) {  // the rest of the vectors, as a group with places left out
+    float x[U * VE];
+#pragma unroll
+    for (int u = 0; u < U; ++u) R.vec(x + u * VE, min(v + u * NT, R.vecs - 1));
+#pragma unroll
+    for (int u = 1; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < VE; ++e)
+        x[u * VE + e] = v + u * NT < R.vecs ? x[u * VE + e] : -INFINITY;
+    own.add<U * VE>(x, index);
   }
   if (tid < R.tail) {
-    const float x = R.at(A.vocab - R.tail + tid);
-    own.add<1>(&x, A.vocab - R.tail + tid);
+    const int i = A.vocab - R.tail + tid;
+    const float x = R.at(i);
+    own.add<1>(&x, [&](int) { return i; });
   }
-  const float best = reduce<NT>(own.m, [](float a, float b) { return fmaxf(a, b); });
-  double S = 0, T = 0;
-  if (own.S != 0) {
-    const float shift = own.m - best;
-    const double f = expf(shift);
-    S = f * own.S;
-    T = f * (own.T + own.S * shift);
-  }
+  // the row's maximum, then S and T against it
+  __shared__ float wave_m[NW];
+  __shared__ double wave_s[NW], wave_t[NW];
+  const float w_m = wave_reduce(own.m, [](float a, float b) { return fmaxf(a, b); });
+  if (lane == 0) wave_m[wave] = w_m;
+  __syncthreads();
+  float best = wave_m[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) best = fmaxf(best, wave_m[w]);
+  const float shift = fmaxf(own.m - best, -3.402823466e38f);
+  const double f = __builtin_amdgcn_exp2f(shift * 1.44269504f);
   const auto sum = [](double a, double b) { return a + b; };
-  S = reduce<NT>(S, sum);
-  T = reduce<NT>(T, sum);
+  const double w_s = wave_reduce(f * own.S, sum);
+  const double w_t = wave_reduce(f * fma(own.S, (double)shift, own.T), sum);
+  if (lane == 0) {
+    wave_s[wave] = w_s;
+    wave_t[wave] = w_t;
+  }
+  __syncthreads();
+  double S = wave_s[0], T = wave_t[0];
+#pragma unroll
+  for (int w = 1; w < NW; ++w) {
+    S += wave_s[w];
+    T += wave_t[w];
+  }
   const double log_s = log(S);
   if (tid == 0) {
-    const int64_t tok = A.tokens[blockIdx.x];
-    const bool in = tok >= 0 && tok < A.vocab;
-    A.logprob[blockIdx.x] = in ? (float)((double)(R.at((int)tok) - best) - log_s) : NAN;
+    A.logprob[blockIdx.x] = in ? (float)((double)(x_tok - best) - log_s) : NAN;
     A.entropy[blockIdx.x] = (float)(log_s - T / S);
   }
   if (A.top == 0) return;
   int64_t* ids = A.ids + (int64_t)blockIdx.x * A.top;
   float* lps = A.top_logprobs + (int64_t)blockIdx.x * A.top;
 
-  __shared__ uint64_t heads[NT];         // each wave's best keys, descending
+  __shared__ uint64_t heads[NT];  // the threads' best keys
   __shared__ uint64_t found[kCandidates];
-  __shared__ uint64_t bound;
   __shared__ int n_found;
   bool plain = S != S;  // a row with NaN or +inf: the threads' maxima do not order it
   if (!plain) {
-    const uint64_t mine = own.first < 0 ? 0 : key_of(own.m, own.first);
-    uint64_t k = mine;  // sorted over the wave, descending
-#pragma unroll
-    for (int size = 2; size <= 64; size <<= 1)
-#pragma unroll
-      for (int o = size >> 1; o > 0; o >>= 1) {
-        const uint64_t other = shfl_xor64(k, o);
-        const bool greater = ((lane & o) == 0) == ((lane & size) == 0);
-        k = greater ? (k > other ? k : other) : (k < other ? k : other);
-      }
-    heads[tid] = k;
-    if (tid == 0) {
-      n_found = 0;
-      bound = 0;
+    uint64_t k = 0;
+    if (own.first >= 0) {
+      k = key_of(own.m, own.first);
+    } else {  // nothing above −inf: its first element
+      const int first = tid < R.peel ? tid
+                        : tid < R.vecs ? R.peel + tid * VE
+                        : tid < R.tail ? A.vocab - R.tail + tid : -1;
+      if (first >= 0) k = key_of(-INFINITY, first);
     }
-    __syncthreads();
-    if (lane < A.top && k) {  // its rank among all waves' keys
-      int rank = lane;
-      for (int w = 0; w < NW; ++w) {
-        if (w == wave) continue;
-        int lo = 0, hi = 64;
-        while (lo < hi) {
-          const int mid = (lo + hi) >> 1;
-          if (heads[w * 64 + mid] > k) lo = mid + 1;
-          else hi = mid;
-        }
-        rank += lo;
+    if (tid == 0) n_found = 0;
+    sort_wave<64>(k, lane);
+    merge_waves<NW>(k, heads, wave, lane);
+    const uint64_t least = heads[A.top - 1];
+    const auto keep = [&](float x, int i) {
+      const uint64_t c = key_of(x, i);
+      if (c >= least) {
+        const int at = atomicAdd(&n_found, 1);
+        if (at < kCandidates) found[at] = c;
       }
-      if (rank == A.top - 1) bound = k;
-    }
-    __syncthreads();
-    const uint64_t least = bound;
-    if (mine && mine >= least) {
-      auto keep = [&](float x, int i) {
-        const uint64_t c = key_of(x, i);
-        if (c >= least) {
-          const int at = atomicAdd(&n_found, 1);
-          if (at < kCandidates) found[at] = c;
-        }
-      };
-      if (tid < R.peel) keep(R.at(tid), tid);
-#pragma unroll 4
-      for (int u = tid; u < R.vecs; u += NT) {
+    };
+    // each of the threads that reach it, by a wave
+    for (int r = wave; r < A.top; r += NW) {
+      const uint64_t head = heads[r];
+      if (head == 0) break;
+      const int i = index_of(head), vec = (i - R.peel) / VE;
+      const int t = i < R.peel ? i : vec < R.vecs ? vec % NT : i - (A.vocab - R.tail);
+      if (lane == 0 && t < R.peel) keep(R.at(t), t);
+      if (lane == 1 && t < R.tail) keep(R.at(A.vocab - R.tail + t), A.vocab - R.tail + t);
+      for (int u = t + lane * NT; u < R.vecs; u += 64 * NT) {
         float x[VE];
         R.vec(x, u);
 #pragma unroll
         for (int e = 0; e < VE; ++e) keep(x[e], R.peel + u * VE + e);
       }
-      if (tid < R.tail) keep(R.at(A.vocab - R.tail + tid), A.vocab - R.tail + tid);
     }
     __syncthreads();
     const int n = n_found;
@@ -272,7 +341,13 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs A) {
         const uint64_t c = key_of(R.at(i), i);
         if (c < last && c > k) k = c;
       }
-      last = reduce<NT>(k, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+      const auto larger = [](uint64_t a, uint64_t b) { return a > b ? a : b; };
+      k = wave_reduce(k, larger);
+      __syncthreads();
+      if (lane == 0) heads[wave] = k;
+      __syncthreads();
+      last = heads[0];
+      for (int w = 1; w < NW; ++w) last = larger(last, heads[w]);
       if (tid == 0) {
         ids[r] = index_of(last);
         lps[r] = (float)((double)(R.at(index_of(last)) - best) - log_s);
