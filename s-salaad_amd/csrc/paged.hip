@@ -269,7 +269,9 @@ __global__ __launch_bounds__(256) void free_refs_kernel(PagedCache C, PagesArgs 
 
 // fork, launch 1: workgroup 0 settles each fork (work[i]: the page its partly
 // filled one is copied into, -1 where none is needed, -2 where it is refused);
-// the others copy the state.
+// the others copy the state. kPlanThreads forks at a time: a wave checks a fork,
+// its lanes the forks named before and the pages of the source; then the forks
+// that need a page are ranked, and the lowest free pages, 4 a thread at a time.
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PagedCache C, PagesArgs A) {
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
@@ -281,43 +283,55 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PagedCache C, P
     copy_ints(A.refs_out, A.refs, C.pages, i0, step);
     return;
   }
-  // which forks stand, and which of them need a page (the r-th of those: its
-  // index kept in work[n + r])
-  int needed = 0;
+  constexpr int kRefused = -2, kNone = -1, kNeeds = -3;
+  __shared__ int state[kPlanThreads], fresh[kPlanThreads];
+  const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int taken = 0;  // free pages the forks before this run were given
   for (int base = 0; base < A.n; base += kPlanThreads) {
-    const int i = base + tid;
-    bool good = false;
-    int part = 0;
-    if (i < A.n) {
-      const int s = A.src[i], d = A.dst[i];
-      good = s >= 0 && s < C.seqs && d >= 0 && d < C.seqs;
-      if (good) {
+    const int count = min(A.n - base, kPlanThreads);
+    for (int k = wave; k < count; k += kPlanThreads / 64) {
+      const int s = A.src[base + k], d = A.dst[base + k];
+      bool bad = s < 0 || s >= C.seqs || d < 0 || d >= C.seqs;
+      int part = 0;
+      if (!bad) {
         const int len = A.lengths[s];
-        good = A.lengths[d] == 0 && len >= 0 && len <= C.cols * C.page;
-        for (int j = 0; good && j < i; ++j) good = A.dst[j] != d;
-        for (int c = 0; good && c < (len + C.page - 1) >> C.log2_page; ++c)
-          good = C.has(C.table[(int64_t)s * C.table_stride + c]);
+        bad = A.lengths[d] != 0 || len < 0 || len > C.cols * C.page;
+        const int pages = bad ? 0 : (len + C.page - 1) >> C.log2_page;
+        for (int j = lane; j < base + k; j += 64) bad |= A.dst[j] == d;
+        for (int c = lane; c < pages; c += 64)
+          bad |= !C.has(C.table[(int64_t)s * C.table_stride + c]);
         part = len & (C.page - 1);
       }
-      A.work[i] = good ? -1 : -2;
+      bad = __any(bad);
+      if (lane == 0) state[k] = bad ? kRefused : part ? kNeeds : kNone;
     }
-    int total;
-    const int rank = needed + scan_exclusive(good && part > 0, &total);
-    if (good && part > 0) A.work[A.n + rank] = i;
-    needed += total;
+    __syncthreads();
+    const int mine = tid < count ? state[tid] : kNone;
+    int need;
+    const int rank = scan_exclusive(mine == kNeeds, &need);
+    int given = 0;  // free pages below the scan's place
+    for (int64_t p0 = 0; p0 < C.pages && given < taken + need; p0 += 4 * kPlanThreads) {
+      int idle[4], n_idle = 0;
+      const int64_t p = p0 + 4 * tid;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) idle[k] = p + k < C.pages && A.refs[p + k] == 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) n_idle += idle[k];
+      int total;
+      int r = given + scan_exclusive(n_idle, &total) - taken;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (idle[k] && r >= 0 && r < need) fresh[r] = (int)(p + k);
+        r += idle[k];
+      }
+      given += total;
+    }
+    __syncthreads();
+    if (tid < count)
+      A.work[base + tid] = mine != kNeeds ? mine : rank < given - taken ? fresh[rank] : kRefused;
+    taken = min(given, taken + need);
+    __syncthreads();
   }
-  __syncthreads();
-  // the lowest free pages, in order, to the forks that need one
-  int given = 0;
-  for (int64_t base = 0; base < C.pages && given < needed; base += kPlanThreads) {
-    const int64_t p = base + tid;
-    const bool idle = p < C.pages && A.refs[p] == 0;
-    int total;
-    const int rank = given + scan_exclusive(idle, &total);
-    if (idle && rank < needed) A.work[A.work[A.n + rank]] = (int)p;
-    given += total;
-  }
-  for (int r = given + tid; r < needed; r += kPlanThreads) A.work[A.work[A.n + r]] = -2;
 }
 
 // fork, launch 2: workgroup (x, fork): the fork's row, length and references
@@ -488,7 +502,7 @@ extern "C" int ssl_pages_free(const ssl_pages_args* a, void* stream) {
   return check_hip(hipGetLastError(), "pages_free launch");
 }
 
-extern "C" int64_t ssl_pages_fork_workspace_size(int64_t n) { return n > 0 ? 8 * n : 0; }
+extern "C" int64_t ssl_pages_fork_workspace_size(int64_t n) { return n > 0 ? 4 * n : 0; }
 
 extern "C" int ssl_pages_fork(const ssl_pages_args* a, void* stream) {
   clear_error();

@@ -328,7 +328,7 @@ def fork_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
     n = src.shape[0]
     lengths_out = torch.empty_like(lengths)
     ok = torch.empty(n, dtype=torch.bool, device=dev)
-    need = 8 * n  # ssl_pages_fork_workspace_size
+    need = _lib.load().ssl_pages_fork_workspace_size(n)
     work = torch.empty(need, dtype=torch.uint8, device=dev)
     _call("ssl_pages_fork", _PAGES.pack(
         _PAGES.size, *pools, *_grid(table), _lib.dtype_code(k_pool.dtype), lengths.data_ptr(),

@@ -437,6 +437,52 @@ def test_fork_of_missing_pages_and_one_layer(gpu_device):
     assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
 
 
+def test_many_forks_and_pages(gpu_device):
+    """More forks and pages than one workgroup holds at a time, and more forks
+    than free pages."""
+    import ssalaad_amd as sa
+
+    dev, n, page = gpu_device, 2500, 16
+    g = torch.Generator().manual_seed(13)
+    pages = 9000
+    order = torch.randperm(pages, generator=g).int()
+    table = torch.full((2 * n, 1), -1, dtype=torch.int32)
+    table[:n, 0] = order[:n]
+    lens = torch.zeros(2 * n, dtype=torch.int32)
+    lens[:n] = torch.randint(0, 17, (n,), generator=g).int()
+    table[:n][lens[:n] == 0] = -1
+    refs = torch.zeros(pages, dtype=torch.int32)
+    refs[table[table >= 0].long()] = 1
+    refs[order[n: pages - 1200].long()] = 1  # others hold these: too few are free
+    kp, vp = pc.cache(pages, 1, page, 64, torch.bfloat16, g, layers=1)
+    src = torch.randperm(n, generator=g)
+    dst = n + torch.randperm(n, generator=g)
+    kd, vd = kp.to(dev), vp.to(dev)
+    got = sa.fork_pages(table.to(dev), lens.to(dev), refs.to(dev), kd, vd, src.int().to(dev),
+                        dst.int().to(dev))
+    part = lens[src].long() % page
+    need = part > 0
+    free = (refs == 0).nonzero()[:, 0]
+    rank = need.long().cumsum(0) - 1
+    ok = ~need | (rank < free.numel())
+    assert need.sum() > free.numel() > 1024
+    t, ln, r = table.clone(), lens.clone(), refs.clone()
+    i = (ok & need).nonzero()[:, 0]
+    fresh = free[rank[i]]
+    t[dst[i], 0] = fresh.int()
+    r[fresh] = 1
+    whole = (ok & ~need & (lens[src] > 0)).nonzero()[:, 0]
+    t[dst[whole], 0] = table[src[whole], 0]
+    r[table[src[whole], 0].long()] += 1
+    ln[dst[ok]] = lens[src[ok]]
+    for a, b in zip(got, (t, ln, r, ok)):
+        assert torch.equal(a.cpu(), b)
+    keep = torch.arange(page) < part[i, None]
+    for a, b in ((kd, kp), (vd, vp)):
+        b[0, fresh] = torch.where(keep[:, None, :, None], b[0, table[src[i], 0].long()], b[0, fresh])
+        assert torch.equal(a.cpu(), b)
+
+
 @pytest.mark.parametrize("pages", [1, 5, 64, 1023, 2500])
 @pytest.mark.parametrize("share", [0.0, 0.1, 0.6, 1.0])
 def test_compact_moves_the_pages_in_use_down(pages, share, gpu_device):

@@ -100,8 +100,9 @@ def test_page_arguments_are_checked_before_any_launch():
         assert _try(fn, st, base, _8=0) == 1 and getattr(lib, fn)(None, None) == 1
         for i in needed:
             assert _try(fn, st, base, **{f"_{i}": 0}) == 1, (fn, i)
-    assert lib.ssl_pages_fork_workspace_size(5) == 40 and lib.ssl_pages_fork_workspace_size(0) == 0
-    assert _try("ssl_pages_fork", st, base, _28=15) == 3 and _try("ssl_pages_fork", st, base, _27=0) == 3
+    need = lib.ssl_pages_fork_workspace_size(2)
+    assert need > 0 and lib.ssl_pages_fork_workspace_size(0) == 0
+    assert _try("ssl_pages_fork", st, base, _28=need - 1) == 3 and _try("ssl_pages_fork", st, base, _27=0) == 3
     need = lib.ssl_pages_compact_workspace_size(9)
     assert need > 0 and _try("ssl_pages_compact", st, base, _28=need - 1) == 3
     assert _try("ssl_pages_compact", st, base, _27=0) == 3
