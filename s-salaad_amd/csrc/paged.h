@@ -43,8 +43,45 @@ struct AttnArgs {
   // split contexts: the most parts of a row and its tiles per part at least,
   // and the parts' outputs, maxima and sums
   int n_split, per;
+  int waves;  // of a workgroup of the kernel for few rows
+  float us;   // the plan's estimate of the call
   float *part_o, *part_ml;
 };
+
+// A sequence's rows of one key/value head: its tokens' query heads, packed token
+// by token (row r: token r / G, head r % G of the group), and their positions.
+struct Chunk {
+  int64_t t0;    // its first token
+  int rows, p0;  // p0: the first token's position
+  __device__ __forceinline__ Chunk(const PagedCache& C, const AttnArgs& A, int s, int G) {
+    int64_t a = s, b = s + 1;
+    if (A.cu) {
+      a = s == 0 ? 0 : A.cu[s];
+      a = min(max(a, (int64_t)0), A.tokens);
+      b = min(max((int64_t)A.cu[s + 1], a), A.tokens);
+    }
+    t0 = a;
+    rows = (int)(b - a) * G;
+    p0 = min(max(A.lengths[s], 0), C.cols << C.log2_page) - (int)(b - a);
+  }
+  // one token a sequence
+  __device__ __forceinline__ Chunk(const PagedCache& C, const AttnArgs& A, int s)
+      : t0(s), rows(A.heads / C.kv_heads),
+        p0(min(max(A.lengths[s], 0), C.cols << C.log2_page) - 1) {}
+};
+
+// Zeros for the heads of key/value head kh of tokens past the last chunk.
+__device__ __forceinline__ void zero_tail(const PagedCache& C, const AttnArgs& A, int kh, int row16,
+                                          int tid, int threads) {
+  const int G = A.heads / C.kv_heads;
+  const int64_t end = min(max((int64_t)A.cu[C.seqs], (int64_t)0), A.tokens);
+  const int64_t n = (A.tokens - end) * G * row16;
+  for (int64_t i = tid; i < n; i += threads) {
+    const int64_t r = i / row16;
+    *(uint4*)(A.out + (((end + r / G) * A.heads + kh * G + r % G) * row16 + i % row16) * 16) =
+        uint4{0, 0, 0, 0};
+  }
+}
 
 // The positions a run of tokens at p_min … p_max of one sequence sees, as tiles
 // of T positions: the first `sink_tiles` of the context, then those from `base`.
@@ -84,9 +121,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
-// One token per sequence (paged_decode.hip), chunks (paged_prompt.hip).
-int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_length);
-int paged_decode_launch(const PagedCache& C, const AttnArgs& A, int dtype, hipStream_t st);
+// Few rows of a key/value head (paged_decode.hip), or many (paged_prompt.hip).
+// The plans fill the split and return the bytes of the parts.
+int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
+                          int64_t max_length);
+int paged_decode_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64_t max_tokens,
+                        hipStream_t st);
 int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
                           int64_t max_length);
 int paged_prompt_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64_t max_tokens,

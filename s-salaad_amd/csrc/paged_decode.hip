@@ -1,18 +1,19 @@
-// Attention of one new token per sequence over its pages.
+// Attention over pages where a key/value head has few rows (query heads of its
+// group times tokens): one new token per sequence, or a few.
 //
-// The keys and values are read once, so memory bounds it: per key 4·head_dim
-// operations a query head on 4·head_dim bytes (16-bit, one head per key/value
-// head). Both products still run on the matrix cores, which take a group of up
-// to 16 query heads at the cost of one, and keep the vector units free:
+// The keys and values are read once for 16 rows, so memory bounds it: per key
+// 4·head_dim operations a row on 4·head_dim bytes (16-bit). Both products still
+// run on the matrix cores, which take 16 rows at the cost of one, and keep the
+// vector units free:
 //
-//   Sᵀ = K·Qᵀ   16 keys × 16 heads a tile. A lane's accumulators are 4 keys of
-//               one head, so a head's maximum needs two exchanges.
+//   Sᵀ = K·Qᵀ   16 keys × 16 rows a tile. A lane's accumulators are 4 keys of
+//               one row, so a row's maximum needs two exchanges.
 //   Oᵀ = Vᵀ·Pᵀ  P as the accumulators leave it: a contraction may take the keys
 //               in any order as long as V's lanes use the same, so neither
 //               operand passes through LDS. A lane reads 16-byte pieces of the
 //               8 (fp32: 4) keys it contracts and transposes them in registers.
 //
-// A wave takes every fourth tile of its workgroup's part of the context and
+// A wave takes every NW-th tile of its workgroup's part of the context and
 // keeps its own running maximum, sum and output; the waves are joined through
 // LDS, the parts of a split context by join_kernel.
 #include <hip/hip_runtime.h>
@@ -21,12 +22,12 @@
 
 #include <algorithm>
 
-#include "paged.h"
+#include "paged_join.h"
 
 namespace ssl {
 namespace {
 
-constexpr int kHeadRows = 16;  // query heads a workgroup takes at most
+constexpr int kRows = 16;  // rows a workgroup takes
 
 template <int DT, int HD>
 struct Shape {
@@ -41,6 +42,12 @@ struct Shape {
   static constexpr int VD = VE * EB / 4;  // dwords of a vector
 };
 
+// Waves of a wide workgroup: as many as its registers allow at once.
+constexpr int wide_waves(int dt, int hd) { return hd == 64 ? 16 : dt == DT_F32 && hd == 256 ? 4 : 8; }
+
+// Rows of a sequence and key/value head at most (tokens of one sequence).
+int64_t max_rows(const AttnArgs& A, int G) { return A.cu ? A.tokens * G : G; }
+
 // VD dwords from a 4·VD-byte aligned address
 template <int VD>
 __device__ __forceinline__ void load_dwords(uint32_t* r, const char* p) {
@@ -53,36 +60,51 @@ __device__ __forceinline__ void load_dwords(uint32_t* r, const char* p) {
   }
 }
 
-template <int DT, int HD>
-__global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode_kernel(PagedCache C, AttnArgs A) {
+// CHUNKS: tokens by cu, each row with a position of its own; else one token a
+// sequence, whose position is a scalar.
+template <int DT, int HD, int NW, bool CHUNKS>
+__global__ __launch_bounds__(NW * 64, NW > 4 ? NW / 4 : DT == DT_F32 && HD == 256 ? 1 : 2)
+void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
   using S = Shape<DT, HD>;
   using M = Mma<DT, S::KE>;
   using Frag = typename M::Frag;
-  extern __shared__ float sh_o[];  // [4][rows][HD]
-  __shared__ float sh_m[4][kHeadRows], sh_l[4][kHeadRows];
+  extern __shared__ float sh_o[];  // [NW][rows][HD]
+  __shared__ float sh_m[NW][kRows], sh_l[NW][kRows];
 
   const int G = A.heads / C.kv_heads;
-  const int n_hb = (G + kHeadRows - 1) / kHeadRows;
-  const int kh = blockIdx.y / n_hb, g0 = (blockIdx.y % n_hb) * kHeadRows;
-  const int rows = min(G - g0, kHeadRows), h0 = kh * G + g0;
-  const int64_t s = blockIdx.z;
+  const int kh = blockIdx.y / n_blocks;
+  const int s = blockIdx.z;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int c = lane & 15, g = lane >> 4;
-
-  const int p = min(A.lengths[s], C.cols << C.log2_page) - 1;
-  const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
-  const TileRange range = tile_range<S::T>(p, p, A.window, A.sinks);
+  if (CHUNKS && s == C.seqs) {
+    if (blockIdx.x == 0 && blockIdx.y % n_blocks == 0)
+      zero_tail(C, A, kh, HD * S::EB / 16, threadIdx.x, NW * 64);
+    return;
+  }
+  const Chunk chunk = CHUNKS ? Chunk(C, A, s, G) : Chunk(C, A, s);
+  const int n_rows = CHUNKS ? chunk.rows : G;
+  for (int block = blockIdx.y % n_blocks; block * kRows < n_rows; block += n_blocks) {
+  const int row_a = block * kRows, rows = min(n_rows - row_a, kRows);
+  // row c and its position; the block's range of them
+  const int r = row_a + min(c, rows - 1);
+  const int64_t token = CHUNKS ? chunk.t0 + r / G : s;
+  const int head = kh * G + (CHUNKS ? r % G : r);
+  const int p_min = CHUNKS ? chunk.p0 + row_a / G : chunk.p0;
+  const int p_max = CHUNKS ? chunk.p0 + (row_a + rows - 1) / G : p_min;
+  const int p = CHUNKS ? chunk.p0 + r / G : p_min;
+  const auto first_of = [&](int q) { return A.window && q + 1 > A.window ? q + 1 - A.window : 0; };
+  const int first = first_of(p), first_min = first_of(p_min), first_max = first_of(p_max);
+  const TileRange range = tile_range<S::T>(max(p_min, 0), p_max, A.window, A.sinks);
   const int per = part_tiles(A, range.count);
   const int lo = blockIdx.x * per, hi = min(lo + per, range.count);
   const bool whole = per >= range.count;
-  if (lo >= hi && blockIdx.x > 0) return;  // the join reads no part past the last
+  if (lo >= hi && blockIdx.x > 0) continue;  // the join reads no part past the last
 
   Frag qf[S::KS];
 #pragma unroll
   for (int i = 0; i < S::KS; ++i)
     qf[i] = load_kfrag<DT, S::KE>(
-        A.q, s * A.q_token + (int64_t)(h0 + min(c, rows - 1)) * A.q_head + (4 * i + g) * S::KE,
-        S::KE);
+        A.q, token * A.q_token + (int64_t)head * A.q_head + (4 * i + g) * S::KE, S::KE);
 
   {
     uint32_t* q = (uint32_t*)qf;
@@ -96,7 +118,7 @@ __global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode
   const uint32_t k_off = c * slot_bytes + g * S::KE * S::EB;
   const uint32_t v_off = 4 * g * slot_bytes + c * S::VE * S::EB;
   const int64_t head_off = kh * C.head_stride;
-  const int32_t* row = C.table + s * C.table_stride;
+  const int32_t* row = C.table + (int64_t)s * C.table_stride;
 
   f32x4 o[S::U * S::VE];
 #pragma unroll
@@ -115,10 +137,10 @@ __global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode
   };
   if (lo + wave < hi) pages_of(lo + wave, page);
 
-  for (int i = lo + wave; i < hi; i += 4) {
+  for (int i = lo + wave; i < hi; i += NW) {
     const int key0 = range.tile(i) * S::T;
     const char *kb[S::NS], *vb[S::NS];
-    bool all = key0 + S::T - 1 <= p && (key0 >= first || key0 + S::T <= A.sinks);
+    bool all = key0 + S::T - 1 <= p_min && (key0 >= first_max || key0 + S::T <= A.sinks);
     bool has[S::NS];
 #pragma unroll
     for (int t = 0; t < S::NS; ++t) {
@@ -143,7 +165,7 @@ __global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode
 #pragma unroll
         for (int w = 0; w < S::U; ++w)
           load_dwords<S::VD>(vr[t][e][w], vb[t] + (size_t)(e * slot_bytes) + v_off + w * 16 * S::VE * S::EB);
-    if (i + 4 < hi) pages_of(i + 4, page);
+    if (i + NW < hi) pages_of(i + NW, page);
     __builtin_amdgcn_sched_barrier(0);
 
     f32x4 acc[S::NS];
@@ -158,14 +180,15 @@ __global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode
     for (int t = 0; t < S::NS; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[t][e] = acc[t][e] * A.scale_log2;
-    if (!all) {  // what is not seen: no weight, and values that may hold anything
+    if (!all) {  // what a row does not see: no weight; what none sees may hold anything
 #pragma unroll
       for (int t = 0; t < S::NS; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int key = key0 + 16 * t + 4 * g + e;
-          const bool see = has[t] && key <= p && (key >= first || key < A.sinks);
-          x[t][e] = see ? x[t][e] : -INFINITY;
+          const bool mine = has[t] && key <= p && (key >= first || key < A.sinks);
+          const bool see = has[t] && key <= p_max && (key >= first_min || key < A.sinks);
+          x[t][e] = mine ? x[t][e] : -INFINITY;
 #pragma unroll
           for (int w = 0; w < S::U; ++w)
 #pragma unroll
@@ -245,24 +268,25 @@ __global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode
       }
   }
   __syncthreads();
-  for (int i = threadIdx.x * 4; i < rows * HD; i += 1024) {
-    const int r = i / HD, d = i % HD;
-    float top = sh_m[0][r];
+  for (int i = threadIdx.x * 4; i < rows * HD; i += NW * 256) {
+    const int k = i / HD, d = i % HD;
+    float top = sh_m[0][k];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, sh_m[w][r]);
+    for (int w = 1; w < NW; ++w) top = fmaxf(top, sh_m[w][k]);
     const float base = top == -INFINITY ? 0.f : top;
     f32x4 acc = {0.f, 0.f, 0.f, 0.f};
     float sum = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float a = exp2f(sh_m[w][r] - base);
-      sum += sh_l[w][r] * a;
-      acc += *(const f32x4*)(sh_o + (w * rows + r) * HD + d) * a;
+    for (int w = 0; w < NW; ++w) {
+      const float a = exp2f(sh_m[w][k] - base);
+      sum += sh_l[w][k] * a;
+      acc += *(const f32x4*)(sh_o + (w * rows + k) * HD + d) * a;
     }
-    const int64_t at = s * A.heads + h0 + r;
+    const int64_t at = CHUNKS
+                           ? (chunk.t0 + (row_a + k) / G) * A.heads + kh * G + (row_a + k) % G
+                           : (int64_t)s * A.heads + kh * G + row_a + k;
     if (whole) {
-      const float inv = sum == 0.f ? 0.f : 1.f / sum;
-      acc *= inv;
+      acc *= sum == 0.f ? 0.f : 1.f / sum;
       if constexpr (DT == DT_F32)
         *(f32x4*)(A.out + (at * HD + d) * 4) = acc;
       else
@@ -277,86 +301,89 @@ __global__ __launch_bounds__(256, DT == DT_F32 && HD == 256 ? 1 : 2) void decode
       }
     }
   }
+  if (!CHUNKS) return;  // n_blocks covers the group
+  __syncthreads();      // the next rows use the same LDS
+  }
 }
 
-// The parts of a split context joined, one workgroup a (token, head): HD / 4
-// lanes take the features, the lane groups every (1024 / HD)-th part.
-template <int DT, int HD>
-__global__ __launch_bounds__(256) void decode_join_kernel(PagedCache C, AttnArgs A) {
-  constexpr int LN = HD / 4, NG = 256 / LN;
-  __shared__ f32x4 sh_o[NG][LN];
-  __shared__ float sh_l[NG];
-  const int64_t s = blockIdx.y, at = s * A.heads + blockIdx.x;
-  const int p = min(A.lengths[s], C.cols << C.log2_page) - 1;
-  const TileRange range = tile_range<Shape<DT, HD>::T>(p, p, A.window, A.sinks);
-  const int per = part_tiles(A, range.count);
-  if (per >= range.count) return;  // the one part wrote the output
-  const int parts = (range.count + per - 1) / per;
-  const int d = threadIdx.x % LN, grp = threadIdx.x / LN;
-  const float* ml = A.part_ml + 2 * at * A.n_split;
-  const float* po = A.part_o + at * A.n_split * HD + 4 * d;
-  float top = -INFINITY;
-  for (int i = threadIdx.x & 63; i < parts; i += 64) top = fmaxf(top, ml[2 * i]);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (int i = grp; i < parts; i += NG) {
-    const float a = exp2f(ml[2 * i] - base);
-    sum += ml[2 * i + 1] * a;
-    acc += *(const f32x4*)(po + (int64_t)i * HD) * a;
-  }
-  sh_o[grp][d] = acc;
-  if (d == 0) sh_l[grp] = sum;
-  __syncthreads();
-  if (grp) return;
-  acc = sh_o[0][d];
-  sum = sh_l[0];
-#pragma unroll
-  for (int i = 1; i < NG; ++i) {
-    acc += sh_o[i][d];
-    sum += sh_l[i];
-  }
-  acc *= sum == 0.f ? 0.f : 1.f / sum;
-  if constexpr (DT == DT_F32)
-    *(f32x4*)(A.out + (at * HD + 4 * d) * 4) = acc;
-  else
-    *(uint2*)(A.out + (at * HD + 4 * d) * 2) =
-        uint2{pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3])};
-}
-
-template <int DT, int HD>
-void launch(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
+template <int DT, int HD, int NW, bool CHUNKS>
+int launch_waves(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
   const int G = A.heads / C.kv_heads;
-  const int n_hb = (G + kHeadRows - 1) / kHeadRows;
-  const size_t lds = 4 * sizeof(float) * HD * std::min(G, kHeadRows);
-  const dim3 grid((unsigned)A.n_split, (unsigned)(C.kv_heads * n_hb), (unsigned)A.tokens);
-  hipLaunchKernelGGL((decode_kernel<DT, HD>), grid, dim3(256), lds, st, C, A);
-  if (A.n_split > 1)
-    hipLaunchKernelGGL((decode_join_kernel<DT, HD>), dim3((unsigned)A.heads, (unsigned)A.tokens),
-                       dim3(256), 0, st, C, A);
+  const int n_blocks = (int)std::max<int64_t>(1, (max_tokens * G + kRows - 1) / kRows);
+  const size_t lds = NW * sizeof(float) * HD * std::min<int64_t>(max_rows(A, G), kRows);
+  if (lds + 4096 > 64 * 1024) {  // beside the static arrays
+    static bool raised[64] = {};  // per device
+    int dev = 0;
+    if (int rc = check_hip(hipGetDevice(&dev), "device query")) return rc;
+    if (dev < 0 || dev >= 64 || !raised[dev]) {
+      if (int rc = check_hip(
+              hipFuncSetAttribute((const void*)decode_kernel<DT, HD, NW, CHUNKS>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize,
+                                  NW * (int)sizeof(float) * HD * kRows),
+              "shared memory size"))
+        return rc;
+      if (dev >= 0 && dev < 64) raised[dev] = true;
+    }
+  }
+  const dim3 grid((unsigned)A.n_split, (unsigned)(C.kv_heads * n_blocks),
+                  (unsigned)(C.seqs + (A.cu ? 1 : 0)));
+  hipLaunchKernelGGL((decode_kernel<DT, HD, NW, CHUNKS>), grid, dim3(NW * 64), lds, st, C, A, n_blocks);
+  if (A.n_split > 1) launch_join<DT, HD, Shape<DT, HD>::T, kRows>(C, A, st);
+  return SSL_OK;
+}
+
+template <int DT, int HD>
+int launch(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
+  constexpr int WIDE = wide_waves(DT, HD);
+  if (A.cu)
+    return A.waves == 4 ? launch_waves<DT, HD, 4, true>(C, A, max_tokens, st)
+                        : launch_waves<DT, HD, WIDE, true>(C, A, max_tokens, st);
+  return A.waves == 4 ? launch_waves<DT, HD, 4, false>(C, A, max_tokens, st)
+                      : launch_waves<DT, HD, WIDE, false>(C, A, max_tokens, st);
 }
 
 template <int DT>
-void launch_dt(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
-  if (C.head_dim == 64) launch<DT, 64>(C, A, st);
-  else if (C.head_dim == 128) launch<DT, 128>(C, A, st);
-  else launch<DT, 256>(C, A, st);
+int launch_dt(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
+  if (C.head_dim == 64) return launch<DT, 64>(C, A, max_tokens, st);
+  if (C.head_dim == 128) return launch<DT, 128>(C, A, max_tokens, st);
+  return launch<DT, 256>(C, A, max_tokens, st);
 }
 
 }  // namespace
 
-// Parts of about 1/2048 of the longest possible work, of 4 tiles (one a wave)
-// at least. Fills n_split and per; returns the parts' bytes.
-int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_length) {
+// One part where a wide workgroup's waves take the longest context in a few
+// steps and the rows' workgroups leave the device room for that many waves (16
+// sequences of 1000 positions, 16 heads of 128: 16 µs, in 8 parts of narrow ones
+// 20; 64 of 300, 8 key/value heads: 11 and 15); else parts of about 1/2048 of
+// the longest possible work, of 4 tiles (one a wave) at least. The estimate: 6 µs
+// and every 16 rows' reading of their context at 7 TB/s, the rate from the caches
+// (2.7 for 256-wide heads, whose registers leave room for half the waves).
+int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
+                          int64_t max_length) {
+  constexpr int kWideTiles = 48;
   const int T = dtype == SSL_F32 ? 16 : 32;
   const int G = A->heads / C.kv_heads;
-  const int64_t blocks = A->tokens * C.kv_heads * ((G + kHeadRows - 1) / kHeadRows);
+  const int64_t blocks = C.seqs * std::max<int64_t>(1, (max_tokens * G + kRows - 1) / kRows) *
+                         C.kv_heads;
   int64_t reach = max_length;
   if (A->window)
-    reach = std::min<int64_t>(reach, (int64_t)A->window + std::min(A->sinks, 0x3fffffff) + 2 * T);
+    reach = std::min<int64_t>(reach, (int64_t)A->window + std::min(A->sinks, 0x3fffffff) +
+                                         (max_tokens > 1 ? kRows : 0) + 2 * T);
   const int64_t tiles = std::max<int64_t>(1, (reach + T - 1) / T);
+  const int64_t rows16 = std::min<int64_t>(blocks, C.kv_heads * (A->tokens * G / kRows + C.seqs));
+  A->us = (float)(6 + (double)rows16 * std::min<int64_t>(reach, std::max<int64_t>(
+                                          max_length - max_tokens / 2, 1)) *
+                          C.head_dim * 2 * elem_bytes(dtype) /
+                          (C.head_dim == 256 ? 2.7e6 : 7e6));
+  const int wide = wide_waves(dtype, C.head_dim);
+  A->n_split = 1;
+  A->per = (int)std::min<int64_t>(tiles, 0x3fffffff);
+  A->waves = 4;
+  if (tiles <= 4) return 0;
+  if (tiles <= kWideTiles && blocks * wide <= 4096) {
+    A->waves = wide;
+    return 0;
+  }
   int64_t per = std::max<int64_t>(4, (tiles * blocks + 2047) / 2048);
   per = (per + 3) / 4 * 4;
   A->per = (int)std::min<int64_t>(per, 0x3fffffff);
@@ -365,11 +392,13 @@ int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t m
   return A->tokens * A->heads * (int64_t)A->n_split * (C.head_dim + 2) * 4;
 }
 
-int paged_decode_launch(const PagedCache& C, const AttnArgs& A, int dtype, hipStream_t st) {
-  if (dtype == SSL_F32) launch_dt<DT_F32>(C, A, st);
-  else if (dtype == SSL_BF16) launch_dt<DT_BF16>(C, A, st);
-  else launch_dt<DT_F16>(C, A, st);
-  return check_hip(hipGetLastError(), "paged decode attention launch");
+int paged_decode_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64_t max_tokens,
+                        hipStream_t st) {
+  int rc;
+  if (dtype == SSL_F32) rc = launch_dt<DT_F32>(C, A, max_tokens, st);
+  else if (dtype == SSL_BF16) rc = launch_dt<DT_BF16>(C, A, max_tokens, st);
+  else rc = launch_dt<DT_F16>(C, A, max_tokens, st);
+  return rc ? rc : check_hip(hipGetLastError(), "paged attention launch");
 }
 
 }  // namespace ssl

@@ -27,7 +27,7 @@
 #include <algorithm>
 #include <utility>
 
-#include "paged.h"
+#include "paged_join.h"
 
 namespace ssl {
 namespace {
@@ -123,20 +123,6 @@ __device__ __forceinline__ void unroll(F f) {
   unroll_over(f, std::make_integer_sequence<int, N>{});
 }
 
-// A sequence's rows of one key/value head and their positions.
-struct Chunk {
-  int64_t t0;  // its first token
-  int rows, p0;  // p0: the first token's position
-  __device__ __forceinline__ Chunk(const PagedCache& C, const AttnArgs& A, int s, int G) {
-    int64_t a = s == 0 ? 0 : A.cu[s], b = A.cu[s + 1];
-    a = min(max(a, (int64_t)0), A.tokens);
-    b = min(max(b, a), A.tokens);
-    t0 = a;
-    rows = (int)(b - a) * G;
-    p0 = min(max(A.lengths[s], 0), C.cols << C.log2_page) - (int)(b - a);
-  }
-};
-
 template <int DT, int HD>
 __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCache C, AttnArgs A,
                                                                           int n_tiles) {
@@ -164,13 +150,7 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
 
   if (tail) {
     if (split) return;
-    const int64_t end = min(max((int64_t)A.cu[s], (int64_t)0), A.tokens);
-    const int64_t n = (A.tokens - end) * G * T::CPR;
-    for (int64_t i = tid; i < n; i += T::THREADS) {
-      const int64_t r = i / T::CPR;
-      *(uint4*)(A.out + (((end + r / G) * A.heads + kh * G + r % G) * T::CPR + i % T::CPR) * 16) =
-          uint4{0, 0, 0, 0};
-    }
+    zero_tail(C, A, kh, T::CPR, tid, T::THREADS);
     return;
   }
   const Chunk chunk(C, A, s, G);
@@ -557,62 +537,6 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   }
 }
 
-// The parts of split rows joined, a wave a row.
-template <int DT, int HD>
-__global__ __launch_bounds__(256) void prompt_join_kernel(PagedCache C, AttnArgs A) {
-  using T = Tile<DT, HD>;
-  constexpr int LN = HD / 4, NG = 64 / LN;
-  const int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int64_t t = at / A.heads;
-  if (t >= A.tokens) return;
-  int a = 0, b = C.seqs;  // the sequence: the first whose end lies past t
-  while (a < b) {
-    const int mid = (a + b) >> 1;
-    if (A.cu[mid + 1] > t) b = mid;
-    else a = mid + 1;
-  }
-  if (a >= C.seqs) return;
-  const int G = A.heads / C.kv_heads;
-  const Chunk chunk(C, A, a, G);
-  const int r = (int)(t - chunk.t0) * G + (int)(at % A.heads) % G;
-  if (r < 0 || r >= chunk.rows) return;
-  const int row_a = r / T::ROWS * T::ROWS, row_b = min(row_a + T::ROWS, chunk.rows) - 1;
-  const TileRange range = tile_range<T::KT>(max(chunk.p0 + row_a / G, 0), chunk.p0 + row_b / G,
-                                            A.window, A.sinks);
-  const int per = part_tiles(A, range.count);
-  if (per >= range.count) return;
-  const int parts = (range.count + per - 1) / per;
-  const int d = lane % LN, grp = lane / LN;
-  const float* ml = A.part_ml + 2 * at * A.n_split;
-  const float* po = A.part_o + at * A.n_split * HD + 4 * d;
-  float top = -INFINITY;
-  for (int i = lane; i < parts; i += 64) top = fmaxf(top, ml[2 * i]);
-#pragma unroll
-  for (int o = 1; o < 64; o <<= 1) top = fmaxf(top, __shfl_xor(top, o));
-  const float base = top == -INFINITY ? 0.f : top;
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (int i = grp; i < parts; i += NG) {
-    const float x = exp2f(ml[2 * i] - base);
-    sum += ml[2 * i + 1] * x;
-    acc += *(const f32x4*)(po + (int64_t)i * HD) * x;
-  }
-#pragma unroll
-  for (int o = LN; o < 64; o <<= 1) {
-    sum += __shfl_xor(sum, o);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) acc[e] += __shfl_xor(acc[e], o);
-  }
-  if (grp) return;
-  acc *= sum == 0.f ? 0.f : 1.f / sum;
-  if constexpr (DT == DT_F32)
-    *(f32x4*)(A.out + (at * HD + 4 * d) * 4) = acc;
-  else
-    *(uint2*)(A.out + (at * HD + 4 * d) * 2) =
-        uint2{pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3])};
-}
-
 int64_t row_tiles(const AttnArgs& A, int G, int64_t max_tokens) {
   return std::max<int64_t>(1, (max_tokens * G + 127) / 128);
 }
@@ -638,11 +562,7 @@ int launch(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream
   }
   hipLaunchKernelGGL((prompt_kernel<DT, HD>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS, st, C,
                      A, (int)n_tiles);
-  if (A.n_split > 1) {
-    const int64_t rows = A.tokens * A.heads;
-    hipLaunchKernelGGL((prompt_join_kernel<DT, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0,
-                       st, C, A);
-  }
+  if (A.n_split > 1) launch_join<DT, HD, T::KT, T::ROWS>(C, A, st);
   return SSL_OK;
 }
 
@@ -655,24 +575,46 @@ int launch_dt(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStr
 
 }  // namespace
 
-// Contexts are split where the rows' tiles do not fill the device, into parts
-// of 4 tiles at least. Fills n_split and per; returns the parts' bytes.
+// Splits contexts where that is faster by an estimate of the launch: a round
+// (a tile a team) takes kRound µs, the rows' workgroups run a device full at a
+// time, and a join costs 4 µs and its parts' traffic at 3 TB/s. (2 prompts of
+// 1000 tokens, 16 heads of 128: whole 23 µs, in 2 parts 38; 500 tokens, 8 fp32
+// heads of 128: whole 74 µs, in 4 parts 35, in 8 32.) Fills n_split and per;
+// returns the parts' bytes.
 int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
                           int64_t max_length) {
-  const int KT = dtype == SSL_F32 ? 32 : 64;
-  const int G = A->heads / C.kv_heads;
+  // measured rounds, by head_dim 64, 128, 256
+  static constexpr double kRound[2][3] = {{1.7, 2.2, 2.8}, {3.9, 7.6, 8.9}};
+  const bool f32 = dtype == SSL_F32;
+  const int KT = f32 ? 32 : 64, G = A->heads / C.kv_heads;
+  const int teams = C.head_dim == 256 ? 1 : 2;
+  const double slots = (double)device_cus() * (C.head_dim == 64 ? 2 : 1);
+  const double round = kRound[f32][C.head_dim == 64 ? 0 : C.head_dim == 128 ? 1 : 2];
   const int64_t tiles = std::min<int64_t>(C.seqs * row_tiles(*A, G, max_tokens),
                                           A->tokens * G / 128 + C.seqs);
   const int64_t blocks = std::max<int64_t>(1, tiles * C.kv_heads);
   int64_t reach = max_length;
-  if (A->window)
+  double mean = 1 - 0.5 * max_tokens / std::max<double>(1, max_length);  // of the rows' contexts
+  if (A->window) {
     reach = std::min<int64_t>(reach, (int64_t)A->window + std::min(A->sinks, 0x3fffffff) +
                                          128 / G + 2 * KT);
+    mean = 1;
+  }
   const int64_t keys = std::max<int64_t>(1, (reach + KT - 1) / KT);
-  const int64_t want = std::max<int64_t>(1, 512 / blocks);
-  const int64_t per = std::max<int64_t>(4, (keys + want - 1) / want);
-  A->per = (int)std::min<int64_t>(per, 0x3fffffff);
-  A->n_split = (int)std::max<int64_t>(1, std::min<int64_t>((keys + per - 1) / per, 65535));
+  const double part_us = A->tokens * A->heads * (double)C.head_dim * 8 / 3e6;
+  double best = 0;
+  for (int n = 1; n <= 64 && (n == 1 || n <= keys); n += n < 4 ? 1 : n / 2) {
+    const int64_t per = (keys + n - 1) / n, parts = (keys + per - 1) / per;
+    const double rounds = (double)((per + teams - 1) / teams);
+    const double full = blocks * mean * keys / teams / slots;
+    const double us = round * std::max(rounds, full) + (parts > 1 ? 4 + parts * part_us : 0);
+    if (n == 1 || us < best) {
+      best = us;
+      A->per = (int)std::min<int64_t>(per, 0x3fffffff);
+      A->n_split = (int)parts;
+    }
+  }
+  A->us = (float)(7 + best);
   if (A->n_split <= 1) return 0;
   return A->tokens * A->heads * (int64_t)A->n_split * (C.head_dim + 2) * 4;
 }
