@@ -56,7 +56,10 @@ struct Tile {
   static constexpr int OT = HD / 32;              // output tiles
   // the chunk permutation of row r (of a group of 16)
   __device__ static int swz_k(int r) { return CPR == 8 ? (r >> 1) & 7 : r & 15; }
-  __device__ static int swz_v(int r) { return F32 ? 0 : CPR == 8 ? r & 6 : (r & 7) << 1; }
+  // (V: pairs of chunks; a transposing read takes 4 rows × 2 pairs at a time)
+  __device__ static int swz_v(int r) {
+    return F32 ? 0 : ((CPR == 8 ? r & 2 : (r & 3) << 1) | (r >> 2 & 1)) << 1;
+  }
 };
 
 // 16 bytes a lane from memory into LDS (lane l: lds + OFF + 16·l), zeros past the
