@@ -129,7 +129,6 @@ int paged_decode_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64
                         hipStream_t st);
 int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
                           int64_t max_length);
-int paged_prompt_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64_t max_tokens,
-                        hipStream_t st);
+int paged_prompt_launch(const PagedCache& C, const AttnArgs& A, int dtype, hipStream_t st);
 
 }  // namespace ssl

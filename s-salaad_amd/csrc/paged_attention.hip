@@ -128,5 +128,5 @@ extern "C" int ssl_paged_attention(const ssl_paged_attention_args* a, void* stre
   hipStream_t st = (hipStream_t)stream;
   const int64_t most = a->cu ? std::min<int64_t>(a->max_tokens, a->tokens) : 1;
   return few ? paged_decode_launch(C, A, (int)a->cache.dtype, most, st)
-             : paged_prompt_launch(C, A, (int)a->cache.dtype, most, st);
+             : paged_prompt_launch(C, A, (int)a->cache.dtype, st);
 }

@@ -126,36 +126,84 @@ __device__ __forceinline__ void unroll(F f) {
   unroll_over(f, std::make_integer_sequence<int, N>{});
 }
 
+// The u-th row tile of all chunks, later tiles of their chunks (the longest
+// contexts) first: its sequence and tile, or a sequence of -1 past the last. Each
+// wave finds it by itself, a lane a sequence: N(t), the tiles numbered t or above,
+// by sums over the lanes, the tile number by bisection, the sequence by counting.
+template <int ROWS>
+__device__ __forceinline__ void find_tile(const PagedCache& C, const AttnArgs& A, int G, int u,
+                                          int lane, int* seq, int* tile) {
+  const auto tiles_of = [&](int s) {
+    if (s >= C.seqs) return 0;
+    const int64_t a = s == 0 ? 0 : min(max((int64_t)A.cu[s], (int64_t)0), A.tokens);
+    const int64_t b = min(max((int64_t)A.cu[s + 1], a), A.tokens);
+    return (int)(((b - a) * G + ROWS - 1) / ROWS);
+  };
+  const int first = tiles_of(lane);  // of the first 64 sequences, kept
+  const auto from = [&](int t) {     // N(t)
+    int n = max(first - t, 0);
+    for (int s = 64 + lane; s < C.seqs; s += 64) n += max(tiles_of(s) - t, 0);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
+    return __builtin_amdgcn_readfirstlane(n);
+  };
+  *seq = -1;
+  if (C.seqs == 1) {
+    const int n = __builtin_amdgcn_readfirstlane(first);
+    *tile = n - 1 - u;
+    if (u < n) *seq = 0;
+    return;
+  }
+  if (from(0) <= u) return;
+  int lo = 0, hi = (int)((A.tokens * G + ROWS - 1) / ROWS);  // N(lo) > u >= N(hi)
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (from(mid) > u) lo = mid;
+    else hi = mid;
+  }
+  *tile = lo;
+  int left = u - from(hi);  // chunks with a tile lo before it
+  for (int s0 = 0; s0 < C.seqs; s0 += 64) {
+    const int n = s0 ? tiles_of(s0 + lane) : first;
+    uint64_t has = __ballot(n > lo);
+    const int count = __popcll(has);
+    if (left < count) {
+      for (; left > 0; --left) has &= has - 1;
+      *seq = s0 + __builtin_ctzll(has);
+      return;
+    }
+    left -= count;
+  }
+}
+
 template <int DT, int HD>
 __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCache C, AttnArgs A,
-                                                                          int n_tiles) {
+                                                                          int64_t n_tiles) {
   using T = Tile<DT, HD>;
   extern __shared__ char lds[];
   const int G = A.heads / C.kv_heads;
   // key/value heads fastest (one head's K and V stay in one die's cache where
-  // their number is a multiple of 8), the longest rows' tiles first; then a
-  // workgroup a head for the tokens past the last chunk. (Between the others
-  // those, which end at once, would leave shader engines idle: workgroups go to
-  // the engines in turn.)
+  // their number is a multiple of 8); after the row tiles a workgroup a head for
+  // the tokens past the last chunk. (Workgroups that end at once come last:
+  // between the others they would leave shader engines idle, to which workgroups
+  // go in turn.)
   uint32_t id = blockIdx.x;
   const int kh = id % C.kv_heads;
   id /= C.kv_heads;
   const int split = id % A.n_split;
   id /= A.n_split;
-  const bool tail = id >= (uint32_t)n_tiles * C.seqs;
-  const int s = tail ? C.seqs : id % C.seqs;
-  const int tile0 = tail ? 0 : n_tiles - 1 - (int)(id / C.seqs);
-
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int team = wave >> 2, w = wave & 3;
   const int col = lane & 31, h = lane >> 5;
 
-  if (tail) {
-    if (split) return;
-    zero_tail(C, A, kh, T::CPR, tid, T::THREADS);
+  if (id >= n_tiles) {
+    if (split == 0) zero_tail(C, A, kh, T::CPR, tid, T::THREADS);
     return;
   }
+  int s, tile;
+  find_tile<T::ROWS>(C, A, G, (int)id, lane, &s, &tile);
+  if (s < 0) return;
   const Chunk chunk(C, A, s, G);
   const int32_t* table = C.table + (int64_t)s * C.table_stride;
   const uint32_t slot_bytes = (uint32_t)(C.slot_stride * T::EB);
@@ -164,14 +212,14 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   const uint64_t v_base = (uint64_t)(uintptr_t)C.v + kh * C.head_stride * T::EB;
   constexpr float kBias = DT == DT_F16 ? 4.f : 0.f;  // fp16 weights are kept 16-fold
 
-  for (int tile = tile0; tile * T::ROWS < chunk.rows; tile += n_tiles) {
+  {
     const int row_a = tile * T::ROWS, row_b = min(row_a + T::ROWS, chunk.rows) - 1;
     const int p_min = chunk.p0 + row_a / G, p_max = chunk.p0 + row_b / G;
     const TileRange range = tile_range<T::KT>(max(p_min, 0), p_max, A.window, A.sinks);
     const int per = part_tiles(A, range.count);
     const bool whole = per >= range.count;
     const int lo = split * per, hi = min(lo + per, range.count);
-    if (lo >= hi && split > 0) continue;
+    if (lo >= hi && split > 0) return;
     const int limit = p_max + 1;
     const int w_first = A.window && p_min + 1 > A.window ? p_min + 1 - A.window : 0;
 
@@ -426,7 +474,6 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
     auto missing = [&](int32_t pg) {
       return (uint32_t)__ballot(!C.has(pg)) & ((1u << (T::KT / 16)) - 1);
     };
-    barrier();  // the rows before have left the buffers
     if (rounds > 0) {
       pgv = pages_of(lo + team);
       bad_next = missing(pgv);
@@ -483,7 +530,7 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
         ml[(w * 2 + 1) * 64 + lane] = l;
       }
       barrier();
-      if (team == 1) continue;
+      if (team == 1) return;
       const float m2 = ml[(w * 2) * 64 + lane], l2 = ml[(w * 2 + 1) * 64 + lane];
       const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
       const float a = exp2f(m - base), b = exp2f(m2 - base);
@@ -498,7 +545,7 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
           for (int e = 0; e < 4; ++e) o[d][4 * k + e] = o[d][4 * k + e] * a + y[e] * b;
         }
     }
-    if (r_a + col > row_b) continue;
+    if (r_a + col > row_b) return;
     const int64_t at = token * A.heads + head;
     float inv = 1.f;
     if (whole) {
@@ -540,15 +587,12 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   }
 }
 
-int64_t row_tiles(const AttnArgs& A, int G, int64_t max_tokens) {
-  return std::max<int64_t>(1, (max_tokens * G + 127) / 128);
-}
-
 template <int DT, int HD>
-int launch(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
+int launch(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
   using T = Tile<DT, HD>;
-  const int64_t n_tiles = row_tiles(A, A.heads / C.kv_heads, max_tokens);
-  const int64_t grid = (n_tiles * C.seqs + 1) * A.n_split * C.kv_heads;
+  // row tiles at most: a partly filled one a sequence
+  const int64_t n_tiles = A.tokens * (A.heads / C.kv_heads) / T::ROWS + C.seqs;
+  const int64_t grid = (n_tiles + 1) * A.n_split * C.kv_heads;
   if (grid > 0x7fffffff)
     return fail(SSL_ERR_UNSUPPORTED, "paged_attention: a grid of %lld workgroups", (long long)grid);
   if (T::LDS > 64 * 1024) {
@@ -564,16 +608,16 @@ int launch(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream
     }
   }
   hipLaunchKernelGGL((prompt_kernel<DT, HD>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS, st, C,
-                     A, (int)n_tiles);
+                     A, n_tiles);
   if (A.n_split > 1) launch_join<DT, HD, T::KT, T::ROWS>(C, A, st);
   return SSL_OK;
 }
 
 template <int DT>
-int launch_dt(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStream_t st) {
-  if (C.head_dim == 64) return launch<DT, 64>(C, A, max_tokens, st);
-  if (C.head_dim == 128) return launch<DT, 128>(C, A, max_tokens, st);
-  return launch<DT, 256>(C, A, max_tokens, st);
+int launch_dt(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
+  if (C.head_dim == 64) return launch<DT, 64>(C, A, st);
+  if (C.head_dim == 128) return launch<DT, 128>(C, A, st);
+  return launch<DT, 256>(C, A, st);
 }
 
 }  // namespace
@@ -593,7 +637,7 @@ int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t m
   const int teams = C.head_dim == 256 ? 1 : 2;
   const double slots = (double)device_cus() * (C.head_dim == 64 ? 2 : 1);
   const double round = kRound[f32][C.head_dim == 64 ? 0 : C.head_dim == 128 ? 1 : 2];
-  const int64_t tiles = std::min<int64_t>(C.seqs * row_tiles(*A, G, max_tokens),
+  const int64_t tiles = std::min<int64_t>(C.seqs * std::max<int64_t>(1, (max_tokens * G + 127) / 128),
                                           A->tokens * G / 128 + C.seqs);
   const int64_t blocks = std::max<int64_t>(1, tiles * C.kv_heads);
   int64_t reach = max_length;
@@ -622,12 +666,11 @@ int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t m
   return A->tokens * A->heads * (int64_t)A->n_split * (C.head_dim + 2) * 4;
 }
 
-int paged_prompt_launch(const PagedCache& C, const AttnArgs& A, int dtype, int64_t max_tokens,
-                        hipStream_t st) {
+int paged_prompt_launch(const PagedCache& C, const AttnArgs& A, int dtype, hipStream_t st) {
   int rc;
-  if (dtype == SSL_F32) rc = launch_dt<DT_F32>(C, A, max_tokens, st);
-  else if (dtype == SSL_BF16) rc = launch_dt<DT_BF16>(C, A, max_tokens, st);
-  else rc = launch_dt<DT_F16>(C, A, max_tokens, st);
+  if (dtype == SSL_F32) rc = launch_dt<DT_F32>(C, A, st);
+  else if (dtype == SSL_BF16) rc = launch_dt<DT_BF16>(C, A, st);
+  else rc = launch_dt<DT_F16>(C, A, st);
   return rc ? rc : check_hip(hipGetLastError(), "paged prompt attention launch");
 }
 
