@@ -64,6 +64,9 @@ struct Chunk {
     rows = (int)(b - a) * G;
     p0 = min(max(A.lengths[s], 0), C.cols << C.log2_page) - (int)(b - a);
   }
+  // tokens a … b − 1 of a sequence of `length` positions
+  __device__ __forceinline__ Chunk(const PagedCache& C, int a, int b, int length, int G)
+      : t0(a), rows((b - a) * G), p0(min(max(length, 0), C.cols << C.log2_page) - (b - a)) {}
   // one token a sequence
   __device__ __forceinline__ Chunk(const PagedCache& C, const AttnArgs& A, int s)
       : t0(s), rows(A.heads / C.kv_heads),

@@ -131,49 +131,56 @@ __device__ __forceinline__ void unroll(F f) {
 // wave finds it by itself, a lane a sequence: N(t), the tiles numbered t or above,
 // by sums over the lanes, the tile number by bisection, the sequence by counting.
 template <int ROWS>
-__device__ __forceinline__ void find_tile(const PagedCache& C, const AttnArgs& A, int G, int u,
-                                          int lane, int* seq, int* tile) {
-  const auto tiles_of = [&](int s) {
-    if (s >= C.seqs) return 0;
-    const int64_t a = s == 0 ? 0 : min(max((int64_t)A.cu[s], (int64_t)0), A.tokens);
-    const int64_t b = min(max((int64_t)A.cu[s + 1], a), A.tokens);
-    return (int)(((b - a) * G + ROWS - 1) / ROWS);
+__device__ __forceinline__ Chunk find_tile(const PagedCache& C, const AttnArgs& A, int G, int u,
+                                           int lane, int* seq, int* tile) {
+  struct Span {
+    int a, b;
   };
-  const int first = tiles_of(lane);  // of the first 64 sequences, kept
-  const auto from = [&](int t) {     // N(t)
+  const auto span_of = [&](int s) {
+    const int n = (int)A.tokens;
+    const int a = s == 0 || s >= C.seqs ? 0 : min(max(A.cu[s], 0), n);
+    return Span{a, s >= C.seqs ? 0 : min(max(A.cu[s + 1], a), n)};
+  };
+  const auto tiles_of = [&](Span x) { return ((x.b - x.a) * G + ROWS - 1) / ROWS; };
+  const Span mine = span_of(lane);  // of the first 64 sequences, kept
+  const int length = A.lengths[min(lane, C.seqs - 1)];
+  const int first = tiles_of(mine);
+  const auto from = [&](int t) {  // N(t)
     int n = max(first - t, 0);
-    for (int s = 64 + lane; s < C.seqs; s += 64) n += max(tiles_of(s) - t, 0);
+    for (int s = 64 + lane; s < C.seqs; s += 64) n += max(tiles_of(span_of(s)) - t, 0);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) n += __shfl_xor(n, o);
     return __builtin_amdgcn_readfirstlane(n);
   };
-  *seq = -1;
+  int s = -1;
   if (C.seqs == 1) {
     const int n = __builtin_amdgcn_readfirstlane(first);
     *tile = n - 1 - u;
-    if (u < n) *seq = 0;
-    return;
-  }
-  if (from(0) <= u) return;
-  int lo = 0, hi = (int)((A.tokens * G + ROWS - 1) / ROWS);  // N(lo) > u >= N(hi)
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (from(mid) > u) lo = mid;
-    else hi = mid;
-  }
-  *tile = lo;
-  int left = u - from(hi);  // chunks with a tile lo before it
-  for (int s0 = 0; s0 < C.seqs; s0 += 64) {
-    const int n = s0 ? tiles_of(s0 + lane) : first;
-    uint64_t has = __ballot(n > lo);
-    const int count = __popcll(has);
-    if (left < count) {
-      for (; left > 0; --left) has &= has - 1;
-      *seq = s0 + __builtin_ctzll(has);
-      return;
+    if (u < n) s = 0;
+  } else if (from(0) > u) {
+    int lo = 0, hi = (int)((A.tokens * G + ROWS - 1) / ROWS);  // N(lo) > u >= N(hi)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (from(mid) > u) lo = mid;
+      else hi = mid;
     }
-    left -= count;
+    *tile = lo;
+    int left = u - from(hi);  // chunks with a tile lo before it
+    for (int s0 = 0; s0 < C.seqs && s < 0; s0 += 64) {
+      uint64_t has = __ballot((s0 ? tiles_of(span_of(s0 + lane)) : first) > lo);
+      const int count = __popcll(has);
+      if (left < count) {
+        for (; left > 0; --left) has &= has - 1;
+        s = s0 + __builtin_ctzll(has);
+      }
+      left -= count;
+    }
   }
+  *seq = s;
+  if (s >= 64) return Chunk(C, A, s, G);
+  s = max(s, 0);
+  return Chunk(C, __builtin_amdgcn_readlane(mine.a, s), __builtin_amdgcn_readlane(mine.b, s),
+               __builtin_amdgcn_readlane(length, s), G);
 }
 
 template <int DT, int HD>
@@ -202,9 +209,8 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
     return;
   }
   int s, tile;
-  find_tile<T::ROWS>(C, A, G, (int)id, lane, &s, &tile);
+  const Chunk chunk = find_tile<T::ROWS>(C, A, G, (int)id, lane, &s, &tile);
   if (s < 0) return;
-  const Chunk chunk(C, A, s, G);
   const int32_t* table = C.table + (int64_t)s * C.table_stride;
   const uint32_t slot_bytes = (uint32_t)(C.slot_stride * T::EB);
   const uint64_t page_bytes = (uint64_t)C.page_stride * T::EB;
@@ -236,14 +242,6 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
     const int wfirst_max = A.window && wp_max + 1 > A.window ? wp_max + 1 - A.window : 0;
 
     uint4 qf[T::QS];
-#pragma unroll
-    for (int i = 0; i < T::QS; ++i) {
-      qf[i] = *(const uint4*)(A.q + (token * A.q_token + (int64_t)head * A.q_head) * T::EB +
-                              (2 * i + h) * 16);
-      const uint32_t flip = A.flip & (T::F32 ? 0x80000000u : 0x80008000u);
-      qf[i] = uint4{(qf[i].x & A.keep) ^ flip, (qf[i].y & A.keep) ^ flip,
-                    (qf[i].z & A.keep) ^ flip, (qf[i].w & A.keep) ^ flip};
-    }
     f32x16 o[T::OT];
 #pragma unroll
     for (int i = 0; i < T::OT; ++i)
@@ -481,6 +479,14 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
       unroll<LOADS>(load);
       pgv = pages_of(lo + team + T::TEAMS);
     }
+#pragma unroll
+    for (int i = 0; i < T::QS; ++i) {  // after the first tile's loads, to arrive with them
+      qf[i] = *(const uint4*)(A.q + (token * A.q_token + (int64_t)head * A.q_head) * T::EB +
+                              (2 * i + h) * 16);
+      const uint32_t flip = A.flip & (T::F32 ? 0x80000000u : 0x80008000u);
+      qf[i] = uint4{(qf[i].x & A.keep) ^ flip, (qf[i].y & A.keep) ^ flip,
+                    (qf[i].z & A.keep) ^ flip, (qf[i].w & A.keep) ^ flip};
+    }
     if (!any) {  // a wave without rows only loads
       for (int n = 0; n < rounds; ++n) {
         const int i = lo + n * T::TEAMS + team;
@@ -514,35 +520,40 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
     wait_loads();
     l += __shfl_xor(l, 32);
 
-    // the second team's part joins the first's
+    // The teams' parts are joined, each team half of the output tiles: it leaves
+    // the other's half in LDS and takes its own from there.
+    constexpr int HALF = T::OT / T::TEAMS;
     if constexpr (T::TEAMS == 2) {
       barrier();
-      f32x4* part = (f32x4*)lds;
-      float* ml = (float*)(lds + 4 * T::OT * 4 * 64 * 16);
-      if (team == 1) {
+      f32x4* part = (f32x4*)lds + (w * HALF * 4) * 64 + lane;  // [team][wave][tile][4][lane]
+      float* ml = (float*)(lds + 2 * 4 * HALF * 4 * 64 * 16) + w * 128 + lane;
+      constexpr int STEP = 4 * HALF * 4 * 64;
 #pragma unroll
-        for (int d = 0; d < T::OT; ++d)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            part[((w * T::OT + d) * 4 + k) * 64 + lane] =
-                f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]};
-        ml[(w * 2) * 64 + lane] = m;
-        ml[(w * 2 + 1) * 64 + lane] = l;
-      }
-      barrier();
-      if (team == 1) return;
-      const float m2 = ml[(w * 2) * 64 + lane], l2 = ml[(w * 2 + 1) * 64 + lane];
-      const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
-      const float a = exp2f(m - base), b = exp2f(m2 - base);
-      l = l * a + l2 * b;
-      m = top;
-#pragma unroll
-      for (int d = 0; d < T::OT; ++d)
+      for (int d = 0; d < HALF; ++d)
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const f32x4 y = part[((w * T::OT + d) * 4 + k) * 64 + lane];
+          f32x4 y;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) o[d][4 * k + e] = o[d][4 * k + e] * a + y[e] * b;
+          for (int e = 0; e < 4; ++e) y[e] = team ? o[d][4 * k + e] : o[HALF + d][4 * k + e];
+          part[team * STEP + (d * 4 + k) * 64] = y;
+        }
+      ml[team * 512] = m;
+      ml[team * 512 + 64] = l;
+      barrier();
+      const float m2 = ml[(team ^ 1) * 512], l2 = ml[(team ^ 1) * 512 + 64];
+      const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+      const float a = exp2f(m - base), b = exp2f(m2 - base);
+      // in the order of the teams, so that both halves have one l
+      l = team ? l2 * b + l * a : l * a + l2 * b;
+      m = top;
+#pragma unroll
+      for (int d = 0; d < HALF; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const f32x4 y = part[(team ^ 1) * STEP + (d * 4 + k) * 64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            o[d][4 * k + e] = (team ? o[HALF + d][4 * k + e] : o[d][4 * k + e]) * a + y[e] * b;
         }
     }
     if (r_a + col > row_b) return;
@@ -550,12 +561,16 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
     float inv = 1.f;
     if (whole) {
       inv = l == 0.f ? 0.f : 1.f / l;
-    } else if (h == 0) {
+    } else if (h == 0 && team == 0) {
       float* ml = A.part_ml + 2 * (at * A.n_split + split);
       ml[0] = m;
       ml[1] = l;
     }
-    // 4 adjacent features at a time (fp32, 64 wide: 2)
+    // 4 adjacent features at a time, or one
+    auto put1 = [&](int f, float y) {
+      float* to = whole ? (float*)A.out + at * HD : A.part_o + (at * A.n_split + split) * HD;
+      to[f] = y;
+    };
     auto put = [&](int f, const f32x4 y) {
       if (!whole)
         *(f32x4*)(A.part_o + (at * A.n_split + split) * HD + f) = y;
@@ -566,23 +581,27 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
     };
     if constexpr (!T::F32) {
 #pragma unroll
-      for (int d = 0; d < T::OT; ++d)
+      for (int d = 0; d < HALF; ++d)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          put(32 * d + 8 * k + 4 * h, f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2],
-                                            o[d][4 * k + 3]} * inv);
-    } else if constexpr (HD > 64) {
-#pragma unroll
-      for (int d = 0; d < T::OT; d += 4)
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          put(32 * d + 4 * (8 * (e >> 2) + 4 * h + (e & 3)),
-              f32x4{o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]} * inv);
+          put(32 * (team * HALF + d) + 8 * k + 4 * h,
+              f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * inv);
     } else {
+      // fp32: feature f of a lane's vector lies in output tile f, so a team holds
+      // HALF adjacent ones
+      constexpr int VE = std::min(T::OT, 4);
 #pragma unroll
-      for (int e = 0; e < 16; e += 2)
-        put(2 * (8 * (e >> 2) + 4 * h + (e & 3)),
-            f32x4{o[0][e], o[1][e], o[0][e + 1], o[1][e + 1]} * inv);
+      for (int d = 0; d < HALF; d += 4)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int f = 32 * d + VE * (8 * (e >> 2) + 4 * h + (e & 3)) + team * HALF;
+          if constexpr (HALF >= 4) {
+            put(f, f32x4{o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]} * inv);
+          } else {
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) put1(f + i, o[i][e] * inv);
+          }
+        }
     }
   }
 }
