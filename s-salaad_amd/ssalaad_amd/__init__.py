@@ -11,6 +11,7 @@ Drop-in for the S-SALAAD hot path:
   * DecodeEngine / generate: KV-cached greedy decode of a loaded model (ssalaad_amd.decode)
   * paged_append, paged_decode_attention, paged_prompt_attention, free_pages,
     fork_pages, compact_pages: serving from a paged key/value cache (ssalaad_amd.paged)
+  * PagedEngine: a loaded model served from such a cache (ssalaad_amd.paged_engine)
   * token_logprobs: log probabilities of given tokens, entropy, alternatives
     (ssalaad_amd.logprobs)
 All compute runs in the HIP kernels of libssalaad_amd.so; there is no CPU path.
@@ -29,6 +30,7 @@ from .ls_linear import (LRSLinear, LRSLinearChain, LRSLinearGroup, PreparedChain
 from .logprobs import TokenLogprobs, token_logprobs
 from .paged import (compact_pages, fork_pages, free_pages, paged_append, paged_decode_attention,
                     paged_prompt_attention)
+from .paged_engine import PagedEngine
 from .project import block_topk, project_S, project_S_nm, project_nm
 
 __all__ = [
@@ -36,6 +38,7 @@ __all__ = [
     "LRSLinear",
     "LRSLinearChain",
     "LRSLinearGroup",
+    "PagedEngine",
     "PreparedChain",
     "SUPPORTED_BLOCK_SIZES",
     "TokenLogprobs",

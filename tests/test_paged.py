@@ -249,3 +249,18 @@ def test_a_status_becomes_the_exception_of_the_c_abi():
         _lib.completed(_lib.SSL_ERR_HIP, "call")
     t = torch.zeros(1)
     assert _lib.completed(t, "call") is t
+
+
+def test_the_paged_engine_needs_a_gpu_and_a_known_model():
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    from ssalaad_amd import PagedEngine
+
+    kw = dict(vocab_size=32, hidden_size=128, intermediate_size=64, num_hidden_layers=1,
+              num_attention_heads=2, num_key_value_heads=1, max_position_embeddings=32)
+    with pytest.raises(ValueError, match="ROCm GPU"):
+        PagedEngine(LlamaForCausalLM(LlamaConfig(**kw)), max_seqs=1, pages=4)
+    with pytest.raises(ValueError, match="activation"):
+        PagedEngine(LlamaForCausalLM(LlamaConfig(**kw, hidden_act="gelu")), max_seqs=1, pages=4)
+    with pytest.raises(ValueError, match="positive"):
+        PagedEngine(LlamaForCausalLM(LlamaConfig(**kw)), max_seqs=0, pages=4)
