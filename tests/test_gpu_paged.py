@@ -365,6 +365,25 @@ def test_free_takes_references_back(seed, gpu_device):
         assert torch.equal(a.cpu(), b)
 
 
+def test_free_of_a_large_state(gpu_device):
+    import ssalaad_amd as sa
+
+    g = torch.Generator().manual_seed(5)
+    seqs, cols, pages = 5000, 30, 90000
+    table = torch.randint(-3, pages + 2, (seqs, cols), generator=g).int()
+    lens = torch.randint(0, 400, (seqs,), generator=g).int()
+    refs = torch.randint(5, 9, (pages,), generator=g).int()
+    gone = torch.randint(-1, seqs + 1, (700,), generator=g).int()
+    got = sa.free_pages(*(t.to(gpu_device) for t in (table, lens, refs, gone)))
+    rows = gone[(gone >= 0) & (gone < seqs)].long().unique()
+    held = table[rows]
+    held = held[(held >= 0) & (held < pages)].long()
+    refs.index_add_(0, held, torch.full(held.shape, -1, dtype=torch.int32))
+    table[rows], lens[rows] = -1, 0
+    for a, b in zip(got, (table, lens, refs)):
+        assert torch.equal(a.cpu(), b)
+
+
 def _fork(table, lens, refs, pools, src, dst, page):
     """The definition, in host integers."""
     t, n, r, ok = table.clone(), lens.clone(), refs.clone(), []
