@@ -126,8 +126,11 @@ struct Row {
     vecs = (A.vocab - peel) / VE;
     tail = A.vocab - peel - vecs * VE;
   }
-  __device__ __forceinline__ void vec(float* f, int v) const {
-    const uint4 r = *(const uint4*)(x + peel * Elem<DT>::bytes + (int64_t)v * 16);
+  __device__ __forceinline__ uint4 raw(int v) const {
+    return *(const uint4*)(x + peel * Elem<DT>::bytes + (int64_t)v * 16);
+  }
+  __device__ __forceinline__ void vec(float* f, int v) const { unpack(f, raw(v)); }
+  __device__ __forceinline__ static void unpack(float* f, const uint4 r) {
     const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -222,22 +225,29 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs A) {
   }
   int v = tid;
   const auto index = [&](int e) { return R.peel + (v + e / VE * NT) * VE + e % VE; };
-  for (; v + (U - 1) * NT < R.vecs; v += U * NT) {
+  // groups of U vectors, the next one's loads before the work on this one; the
+  // last has places left out
+  uint4 ahead[U];
+  const auto load = [&](int first) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) ahead[u] = R.raw(min(first + u * NT, R.vecs - 1));
+  };
+  if (v < R.vecs) load(v);
+  while (v < R.vecs) {
     float x[U * VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) R.vec(x + u * VE, v + u * NT);
+    for (int u = 0; u < U; ++u) R.unpack(x + u * VE, ahead[u]);
+    const int last = v + (U - 1) * NT;
+    if (v + U * NT < R.vecs) load(v + U * NT);
+    if (last >= R.vecs) {
+#pragma unroll
+      for (int u = 1; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < VE; ++e)
+          x[u * VE + e] = v + u * NT < R.vecs ? x[u * VE + e] : -INFINITY;
+    }
     own.add<U * VE>(x, index);
-  }
-  if (v < R.vecs) {  // the rest of the vectors, as a group with places left out
-    float x[U * VE];
-#pragma unroll
-    for (int u = 0; u < U; ++u) R.vec(x + u * VE, min(v + u * NT, R.vecs - 1));
-#pragma unroll
-    for (int u = 1; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < VE; ++e)
-        x[u * VE + e] = v + u * NT < R.vecs ? x[u * VE + e] : -INFINITY;
-    own.add<U * VE>(x, index);
+    v += U * NT;
   }
   if (tid < R.tail) {
     const int i = A.vocab - R.tail + tid;

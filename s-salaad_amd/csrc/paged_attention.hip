@@ -22,8 +22,10 @@ namespace {
 
 // Rows of one key/value head the kernel for few of them is considered for, which
 // reads a context once for 16. (500 tokens, 8 fp32 heads of 128: 20 µs, the other
-// 32; 8 chunks of 40 over 8000 positions, 16 heads of 64: 54 µs, the other 49.)
-constexpr int kFewRows = 512;
+// 34; 8 chunks of 40 over 8000 positions, 16 heads of 64: 54 µs, the other 50. In
+// 16 bits more rows are never its case: 300 tokens of a group of 4 over 2000
+// positions 26 µs, the other 20.)
+constexpr int few_rows(int dtype) { return dtype == SSL_F32 ? 4096 : 512; }
 
 // Checks the arguments and fills the kernels' form of them; `need` receives the
 // workspace the call takes, `few` which kernel.
@@ -84,7 +86,7 @@ int attention_args(const ssl_paged_attention_args* a, PagedCache* C, AttnArgs* A
   *few = !a->cu;
   if (a->cu) {
     *need = paged_prompt_plan(*C, A, dtype, most, reach);
-    if (rows <= kFewRows && C->seqs < 65535 && C->kv_heads * ((rows + 15) / 16) <= 65535) {
+    if (rows <= few_rows(dtype) && C->seqs < 65535 && C->kv_heads * ((rows + 15) / 16) <= 65535) {
       AttnArgs other = *A;
       const int64_t bytes = paged_decode_plan(*C, &other, dtype, most, reach);
       if (other.us <= A->us) {

@@ -351,16 +351,16 @@ int launch_dt(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hipStr
 
 }  // namespace
 
-// One part where a wide workgroup's waves take the longest context in a few
-// steps and the rows' workgroups leave the device room for that many waves (16
+// One part where a wide workgroup's waves take the longest context in 3 steps,
+// or in 6 where there are workgroups enough to keep the device busy meanwhile (16
 // sequences of 1000 positions, 16 heads of 128: 16 µs, in 8 parts of narrow ones
 // 20; 64 of 300, 8 key/value heads: 11 and 15); else parts of about 1/2048 of
 // the longest possible work, of 4 tiles (one a wave) at least. The estimate: 6 µs
 // and every 16 rows' reading of their context at 7 TB/s, the rate from the caches
-// (2.7 for 256-wide heads, whose registers leave room for half the waves).
+// (2.7 for 256-wide heads, whose registers leave room for half the waves), or
+// their products at 80 TFLOP/s in fp32.
 int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
                           int64_t max_length) {
-  constexpr int kWideTiles = 48;
   const int T = dtype == SSL_F32 ? 16 : 32;
   const int G = A->heads / C.kv_heads;
   const int64_t blocks = C.seqs * std::max<int64_t>(1, (max_tokens * G + kRows - 1) / kRows) *
@@ -371,16 +371,17 @@ int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t m
                                          (max_tokens > 1 ? kRows : 0) + 2 * T);
   const int64_t tiles = std::max<int64_t>(1, (reach + T - 1) / T);
   const int64_t rows16 = std::min<int64_t>(blocks, C.kv_heads * (A->tokens * G / kRows + C.seqs));
-  A->us = (float)(6 + (double)rows16 * std::min<int64_t>(reach, std::max<int64_t>(
-                                          max_length - max_tokens / 2, 1)) *
-                          C.head_dim * 2 * elem_bytes(dtype) /
-                          (C.head_dim == 256 ? 2.7e6 : 7e6));
+  const double read = (double)rows16 * C.head_dim *
+                      std::min<int64_t>(reach, std::max<int64_t>(max_length - max_tokens / 2, 1));
+  A->us = (float)(6 + std::max(read * 2 * elem_bytes(dtype) / (C.head_dim == 256 ? 2.7e6 : 7e6),
+                               dtype == SSL_F32 ? read * 4 * kRows / 80e6 : 0.));
   const int wide = wide_waves(dtype, C.head_dim);
   A->n_split = 1;
   A->per = (int)std::min<int64_t>(tiles, 0x3fffffff);
   A->waves = 4;
   if (tiles <= 4) return 0;
-  if (tiles <= kWideTiles && blocks * wide <= 4096) {
+  const int64_t steps = (tiles + wide - 1) / wide;
+  if (wide > 4 && blocks * wide <= 4096 && (steps <= 3 || (steps <= 6 && blocks >= 128))) {
     A->waves = wide;
     return 0;
   }
