@@ -365,6 +365,27 @@ def test_free_takes_references_back(seed, gpu_device):
         assert torch.equal(a.cpu(), b)
 
 
+@pytest.mark.parametrize("seqs,cols,pages", [
+    (1, 1, 1), (4096, 1, 4096), (32, 128, 4095), (1024, 4, 4097), (4097, 1, 300), (3, 0, 5), (0, 4, 7)])
+def test_free_at_the_edge_of_a_small_state(seqs, cols, pages, gpu_device):
+    import ssalaad_amd as sa
+
+    g = torch.Generator().manual_seed(6)
+    wide = torch.randint(-2, pages + 2, (seqs, cols + 3), generator=g).int()
+    lens = torch.randint(0, 400, (seqs,), generator=g).int()
+    refs = torch.randint(5, 9, (pages,), generator=g).int()
+    gone = torch.randint(-1, seqs + 1, (2 * seqs // 3 + 1,), generator=g).int()
+    got = sa.free_pages(wide.to(gpu_device)[:, :cols], *(t.to(gpu_device) for t in (lens, refs, gone)))
+    table = wide[:, :cols].clone()
+    rows = gone[(gone >= 0) & (gone < seqs)].long().unique()
+    held = table[rows]
+    held = held[(held >= 0) & (held < pages)].long()
+    refs.index_add_(0, held, torch.full(held.shape, -1, dtype=torch.int32))
+    table[rows], lens[rows] = -1, 0
+    for a, b in zip(got, (table, lens, refs)):
+        assert torch.equal(a.cpu(), b)
+
+
 def test_free_of_a_large_state(gpu_device):
     import ssalaad_amd as sa
 
