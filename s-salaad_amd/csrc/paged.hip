@@ -7,10 +7,11 @@
 //               a partly filled last page copied
 //   compact     the pages in use moved to the lowest page numbers
 //
-// The page operations are two launches each: the first settles which pages are
-// taken (one workgroup ranks them; others copy the small state arrays), the
-// second moves the data over the whole device. Reference counts change by
-// integer atomics, whose order does not change the result.
+// The page operations are two launches each (freeing in a small state is one):
+// the first settles which pages are taken (one workgroup ranks them; others copy
+// the small state arrays), the second moves the data over the whole device.
+// Reference counts change by integer atomics, whose order does not change the
+// result.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -96,7 +97,10 @@ struct Vec {
 // ---------------------------------------------------------------------------
 // append: a row is one head of one token; LPR lanes hold it, each the VE
 // features from j and their partners from j + HD / 2, so a rotation needs no
-// exchange and a row's loads and stores are whole 16-byte vectors.
+// exchange and a row's loads and stores are whole 16-byte vectors. Memory bounds
+// it, below some hundred tokens the launch: 2048 tokens, 32 + 8 + 8 heads of 128
+// with norms, bf16: 12.0 µs, 4.3 TB/s (a large copy here: 4.83); 16 tokens of 16
+// heads: 4.0 µs.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
   const char *q, *k, *v;
@@ -141,7 +145,8 @@ __global__ __launch_bounds__(256) void append_kernel(PagedCache C, AppendArgs A)
   if (dst < 0) return;
   const void* src = is_q ? A.q : is_v ? A.v : A.k;
   const int64_t off = is_q ? t * A.q_token + head * A.q_head
-                           : is_v ? t * A.v_token + head * A.v_head : t * A.k_token + head * A.k_head;
+                           : is_v ? t * A.v_token + head * A.v_head
+                                  : t * A.k_token + head * A.k_head;
   float a[VE], b[VE];
   Vec<DT>::load(a, src, off + j);
   Vec<DT>::load(b, src, off + j + HD / 2);
@@ -189,7 +194,8 @@ void launch_append(const PagedCache& C, const AppendArgs& A, hipStream_t st) {
   const int rpw = 256 / (C.head_dim / 2 / Vec<DT>::VE);
   const dim3 grid((unsigned)((rows + rpw - 1) / rpw));
   if (C.head_dim == 64) hipLaunchKernelGGL((append_kernel<DT, 64>), grid, dim3(256), 0, st, C, A);
-  else if (C.head_dim == 128) hipLaunchKernelGGL((append_kernel<DT, 128>), grid, dim3(256), 0, st, C, A);
+  else if (C.head_dim == 128)
+    hipLaunchKernelGGL((append_kernel<DT, 128>), grid, dim3(256), 0, st, C, A);
   else hipLaunchKernelGGL((append_kernel<DT, 256>), grid, dim3(256), 0, st, C, A);
 }
 
@@ -384,6 +390,9 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(PagedCache C, P
 
 // fork, launch 2: workgroup (x, fork): the fork's row, length and references
 // (x = 0), and its share of the partly filled page's positions in every layer.
+// 16 forks of sequences of up to 1500 positions, 16 layers of 16 heads of 128,
+// bf16: 9.1 µs beside 5.4 of launch 1. (A wave a head instead of vectors over the
+// device: the whole resampling 34 µs, this way 18.)
 __global__ __launch_bounds__(256) void fork_copy_kernel(PagedCache C, PagesArgs A, int eb) {
   const int i = blockIdx.y;
   const int fresh = A.work[i];
@@ -456,7 +465,9 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PagedCache C
   }
 }
 
-// compact, launch 2: the entries, and the moved pages' data.
+// compact, launch 2: the entries, and the moved pages' data, which bounds the
+// call: 1024 moved pages of 8 layers, 8 heads of 128 and 16 positions, bf16: 216
+// µs, 5.0 TB/s, after 10 of launch 1 over 4096 pages.
 __global__ __launch_bounds__(256) void compact_copy_kernel(PagedCache C, PagesArgs A, int eb) {
   const int64_t P = C.pages;
   const int32_t *from = A.work, *to = A.work + P, *map = A.work + 2 * P;
@@ -485,7 +496,8 @@ __global__ __launch_bounds__(256) void compact_copy_kernel(PagedCache C, PagesAr
 int pages_args(const char* what, const ssl_pages_args* a, bool pools, PagedCache* C, PagesArgs* A) {
   if (!a) return fail(SSL_ERR_INVALID, "%s: no arguments", what);
   if (int rc = paged_cache(what, a->cache, sizeof(ssl_pages_args), pools, C)) return rc;
-  if (a->n < 0 || a->n > 65535) return fail(SSL_ERR_INVALID, "%s: %lld sequences", what, (long long)a->n);
+  if (a->n < 0 || a->n > 65535)
+    return fail(SSL_ERR_INVALID, "%s: %lld sequences", what, (long long)a->n);
   if (!a->refs || !a->refs_out || (C->seqs * (int64_t)C->cols > 0 && !a->table_out))
     return fail(SSL_ERR_INVALID, "%s: null pointer", what);
   *A = PagesArgs{a->lengths, a->refs, a->src, a->dst, (int)a->n, a->table_out, a->lengths_out,

@@ -15,7 +15,14 @@
 //
 // A wave takes every NW-th tile of its workgroup's part of the context and
 // keeps its own running maximum, sum and output; the waves are joined through
-// LDS, the parts of a split context by join_kernel.
+// LDS, the parts of a split context by join_kernel: a second launch, 4 to 5 µs,
+// which a counter in the workspace would save at the price of one that has to be
+// kept at zero between calls.
+//
+// Measured: contexts of up to 60001 positions of 4 sequences, 32 heads over 8 of
+// 128, bf16: 88 µs, 4.86 TB/s (a large copy here: 4.83); 64 sequences, a window of
+// 1024, 16 heads: 94 µs, 4.76 TB/s. One sequence of 717, 16 heads of 64: 7.7 µs, the
+// latency of a launch, of the table, of three loads in turn and of the join of waves.
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
@@ -43,7 +50,9 @@ struct Shape {
 };
 
 // Waves of a wide workgroup: as many as its registers allow at once.
-constexpr int wide_waves(int dt, int hd) { return hd == 64 ? 16 : dt == DT_F32 && hd == 256 ? 4 : 8; }
+constexpr int wide_waves(int dt, int hd) {
+  return hd == 64 ? 16 : dt == DT_F32 && hd == 256 ? 4 : 8;
+}
 
 // Rows of a sequence and key/value head at most (tokens of one sequence).
 int64_t max_rows(const AttnArgs& A, int G) { return A.cu ? A.tokens * G : G; }
@@ -84,225 +93,228 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
   const Chunk chunk = CHUNKS ? Chunk(C, A, s, G) : Chunk(C, A, s);
   const int n_rows = CHUNKS ? chunk.rows : G;
   for (int block = blockIdx.y % n_blocks; block * kRows < n_rows; block += n_blocks) {
-  const int row_a = block * kRows, rows = min(n_rows - row_a, kRows);
-  // row c and its position; the block's range of them
-  const int r = row_a + min(c, rows - 1);
-  const int64_t token = CHUNKS ? chunk.t0 + r / G : s;
-  const int head = kh * G + (CHUNKS ? r % G : r);
-  const int p_min = CHUNKS ? chunk.p0 + row_a / G : chunk.p0;
-  const int p_max = CHUNKS ? chunk.p0 + (row_a + rows - 1) / G : p_min;
-  const int p = CHUNKS ? chunk.p0 + r / G : p_min;
-  const auto first_of = [&](int q) { return A.window && q + 1 > A.window ? q + 1 - A.window : 0; };
-  const int first = first_of(p), first_min = first_of(p_min), first_max = first_of(p_max);
-  const TileRange range = tile_range<S::T>(max(p_min, 0), p_max, A.window, A.sinks);
-  const int per = part_tiles(A, range.count);
-  const int lo = blockIdx.x * per, hi = min(lo + per, range.count);
-  const bool whole = per >= range.count;
-  if (lo >= hi && blockIdx.x > 0) continue;  // the join reads no part past the last
+    const int row_a = block * kRows, rows = min(n_rows - row_a, kRows);
+    // row c and its position; the block's range of them
+    const int r = row_a + min(c, rows - 1);
+    const int64_t token = CHUNKS ? chunk.t0 + r / G : s;
+    const int head = kh * G + (CHUNKS ? r % G : r);
+    const int p_min = CHUNKS ? chunk.p0 + row_a / G : chunk.p0;
+    const int p_max = CHUNKS ? chunk.p0 + (row_a + rows - 1) / G : p_min;
+    const int p = CHUNKS ? chunk.p0 + r / G : p_min;
+    const auto first_of = [&](int q) {
+      return A.window && q + 1 > A.window ? q + 1 - A.window : 0;
+    };
+    const int first = first_of(p), first_min = first_of(p_min), first_max = first_of(p_max);
+    const TileRange range = tile_range<S::T>(max(p_min, 0), p_max, A.window, A.sinks);
+    const int per = part_tiles(A, range.count);
+    const int lo = blockIdx.x * per, hi = min(lo + per, range.count);
+    const bool whole = per >= range.count;
+    if (lo >= hi && blockIdx.x > 0) continue;  // the join reads no part past the last
 
-  Frag qf[S::KS];
-#pragma unroll
-  for (int i = 0; i < S::KS; ++i)
-    qf[i] = load_kfrag<DT, S::KE>(
-        A.q, token * A.q_token + (int64_t)head * A.q_head + (4 * i + g) * S::KE, S::KE);
+    Frag qf[S::KS];
+  #pragma unroll
+    for (int i = 0; i < S::KS; ++i)
+      qf[i] = load_kfrag<DT, S::KE>(
+          A.q, token * A.q_token + (int64_t)head * A.q_head + (4 * i + g) * S::KE, S::KE);
 
-  {
-    uint32_t* q = (uint32_t*)qf;
-    const uint32_t flip = A.flip & (DT == DT_F32 ? 0x80000000u : 0x80008000u);
-#pragma unroll
-    for (int i = 0; i < (int)(sizeof qf / 4); ++i) q[i] = (q[i] & A.keep) ^ flip;
-  }
-
-  // lane offsets within a page's head: key c for K, keys 4g + e for V
-  const uint32_t slot_bytes = (uint32_t)(C.slot_stride * S::EB);
-  const uint32_t k_off = c * slot_bytes + g * S::KE * S::EB;
-  const uint32_t v_off = 4 * g * slot_bytes + c * S::VE * S::EB;
-  const int64_t head_off = kh * C.head_stride;
-  const int32_t* row = C.table + (int64_t)s * C.table_stride;
-
-  f32x4 o[S::U * S::VE];
-#pragma unroll
-  for (int i = 0; i < S::U * S::VE; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // of head c; l: this lane's keys only
-  // fp16 weights are kept 256-fold, so that small ones keep their digits
-  constexpr float kBias = DT == DT_F16 ? 8.f : 0.f;
-
-  // pages of the wave's next tile, read a tile ahead
-  int32_t page[S::NS];
-  auto pages_of = [&](int i, int32_t* pg) {
-    const int key0 = range.tile(min(i, hi - 1)) * S::T;
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t)
-      pg[t] = row[min((key0 + 16 * t) >> C.log2_page, C.cols - 1)];
-  };
-  if (lo + wave < hi) pages_of(lo + wave, page);
-
-  for (int i = lo + wave; i < hi; i += NW) {
-    const int key0 = range.tile(i) * S::T;
-    const char *kb[S::NS], *vb[S::NS];
-    bool all = key0 + S::T - 1 <= p_min && (key0 >= first_max || key0 + S::T <= A.sinks);
-    bool has[S::NS];
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t) {
-      has[t] = C.has(page[t]);
-      all = all && has[t];
-      const int64_t off = ((has[t] ? page[t] : 0) * C.page_stride + head_off +
-                           ((key0 + 16 * t) & (C.page - 1)) * C.slot_stride) * S::EB;
-      kb[t] = C.k + off;
-      vb[t] = C.v + off;
+    {
+      uint32_t* q = (uint32_t*)qf;
+      const uint32_t flip = A.flip & (DT == DT_F32 ? 0x80000000u : 0x80008000u);
+  #pragma unroll
+      for (int i = 0; i < (int)(sizeof qf / 4); ++i) q[i] = (q[i] & A.keep) ^ flip;
     }
-    Frag kf[S::NS][S::KS];
-    uint32_t vr[S::NS][4][S::U][S::VD];
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t)
-#pragma unroll
-      for (int k = 0; k < S::KS; ++k)
-        kf[t][k] = load_kfrag_full<DT, S::KE>(kb[t] + k_off + k * 4 * S::KE * S::EB, 0);
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-#pragma unroll
-        for (int w = 0; w < S::U; ++w)
-          load_dwords<S::VD>(vr[t][e][w], vb[t] + (size_t)(e * slot_bytes) + v_off + w * 16 * S::VE * S::EB);
-    if (i + NW < hi) pages_of(i + NW, page);
-    __builtin_amdgcn_sched_barrier(0);
 
-    f32x4 acc[S::NS];
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t) {
-      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int k = 0; k < S::KS; ++k) M::run(acc[t], kf[t][k], qf[k]);
-    }
-    float x[S::NS][4];
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][e] = acc[t][e] * A.scale_log2;
-    if (!all) {  // what a row does not see: no weight; what none sees may hold anything
-#pragma unroll
+    // lane offsets within a page's head: key c for K, keys 4g + e for V
+    const uint32_t slot_bytes = (uint32_t)(C.slot_stride * S::EB);
+    const uint32_t k_off = c * slot_bytes + g * S::KE * S::EB;
+    const uint32_t v_off = 4 * g * slot_bytes + c * S::VE * S::EB;
+    const int64_t head_off = kh * C.head_stride;
+    const int32_t* row = C.table + (int64_t)s * C.table_stride;
+
+    f32x4 o[S::U * S::VE];
+  #pragma unroll
+    for (int i = 0; i < S::U * S::VE; ++i) o[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;  // of head c; l: this lane's keys only
+    // fp16 weights are kept 256-fold, so that small ones keep their digits
+    constexpr float kBias = DT == DT_F16 ? 8.f : 0.f;
+
+    // pages of the wave's next tile, read a tile ahead
+    int32_t page[S::NS];
+    auto pages_of = [&](int i, int32_t* pg) {
+      const int key0 = range.tile(min(i, hi - 1)) * S::T;
+  #pragma unroll
       for (int t = 0; t < S::NS; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int key = key0 + 16 * t + 4 * g + e;
-          const bool mine = has[t] && key <= p && (key >= first || key < A.sinks);
-          const bool see = has[t] && key <= p_max && (key >= first_min || key < A.sinks);
-          x[t][e] = mine ? x[t][e] : -INFINITY;
-#pragma unroll
-          for (int w = 0; w < S::U; ++w)
-#pragma unroll
-            for (int d = 0; d < S::VD; ++d) vr[t][e][w][d] = see ? vr[t][e][w][d] : 0u;
-        }
-    }
-    float mx = m;
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) mx = fmaxf(mx, x[t][e]);
-    mx = fmaxf(mx, __shfl_xor(mx, 16));
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
-    const float base = (mx == -INFINITY ? 0.f : mx) - kBias;
-    if (__any(mx > m)) {
-      const float a = exp2f(m - (base + kBias));
-      l *= a;
-#pragma unroll
-      for (int k = 0; k < S::U * S::VE; ++k) o[k] *= a;
-    }
-    m = mx;
-#pragma unroll
-    for (int t = 0; t < S::NS; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[t][e] = exp2f(x[t][e] - base);
-        l += x[t][e];
-      }
-    Frag pf;
-    if constexpr (DT == DT_F32) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) pf.f[e] = x[0][e];
-    } else {
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        pf.d[2 * t] = pack2<DT>(x[t][0], x[t][1]);
-        pf.d[2 * t + 1] = pack2<DT>(x[t][2], x[t][3]);
-      }
-    }
-#pragma unroll
-    for (int w = 0; w < S::U; ++w)
-#pragma unroll
-      for (int f = 0; f < S::VE; ++f) {
-        Frag vf;
-        if constexpr (DT == DT_F32) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) vf.f[e] = __uint_as_float(vr[0][e][w][f]);
-        } else {
-#pragma unroll
-          for (int d = 0; d < 4; ++d) {
-            const uint32_t a = vr[d / 2][2 * (d % 2)][w][f / 2];
-            const uint32_t b = vr[d / 2][2 * (d % 2) + 1][w][f / 2];
-            vf.d[d] = __builtin_amdgcn_perm(b, a, f % 2 ? 0x07060302u : 0x05040100u);
-          }
-        }
-        M::run(o[w * S::VE + f], vf, pf);
-      }
-  }
+        pg[t] = row[min((key0 + 16 * t) >> C.log2_page, C.cols - 1)];
+    };
+    if (lo + wave < hi) pages_of(lo + wave, page);
 
-  // join the waves: sums over the lane groups, then o through LDS
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  if (g == 0) {
-    sh_m[wave][c] = m;
-    sh_l[wave][c] = l;
-  }
-  if (c < rows) {
-#pragma unroll
-    for (int w = 0; w < S::U; ++w)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float* to = sh_o + (wave * rows + c) * HD + w * 16 * S::VE + (4 * g + e) * S::VE;
-#pragma unroll
-        for (int f = 0; f < S::VE; f += 4)
-          *(f32x4*)(to + f) = f32x4{o[w * S::VE + f][e], o[w * S::VE + f + 1][e],
-                                    o[w * S::VE + f + 2][e], o[w * S::VE + f + 3][e]};
+    for (int i = lo + wave; i < hi; i += NW) {
+      const int key0 = range.tile(i) * S::T;
+      const char *kb[S::NS], *vb[S::NS];
+      bool all = key0 + S::T - 1 <= p_min && (key0 >= first_max || key0 + S::T <= A.sinks);
+      bool has[S::NS];
+  #pragma unroll
+      for (int t = 0; t < S::NS; ++t) {
+        has[t] = C.has(page[t]);
+        all = all && has[t];
+        const int64_t off = ((has[t] ? page[t] : 0) * C.page_stride + head_off +
+                             ((key0 + 16 * t) & (C.page - 1)) * C.slot_stride) * S::EB;
+        kb[t] = C.k + off;
+        vb[t] = C.v + off;
       }
-  }
-  __syncthreads();
-  for (int i = threadIdx.x * 4; i < rows * HD; i += NW * 256) {
-    const int k = i / HD, d = i % HD;
-    float top = sh_m[0][k];
-#pragma unroll
-    for (int w = 1; w < NW; ++w) top = fmaxf(top, sh_m[w][k]);
-    const float base = top == -INFINITY ? 0.f : top;
-    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      const float a = exp2f(sh_m[w][k] - base);
-      sum += sh_l[w][k] * a;
-      acc += *(const f32x4*)(sh_o + (w * rows + k) * HD + d) * a;
+      Frag kf[S::NS][S::KS];
+      uint32_t vr[S::NS][4][S::U][S::VD];
+  #pragma unroll
+      for (int t = 0; t < S::NS; ++t)
+  #pragma unroll
+        for (int k = 0; k < S::KS; ++k)
+          kf[t][k] = load_kfrag_full<DT, S::KE>(kb[t] + k_off + k * 4 * S::KE * S::EB, 0);
+  #pragma unroll
+      for (int t = 0; t < S::NS; ++t)
+  #pragma unroll
+        for (int e = 0; e < 4; ++e)
+  #pragma unroll
+          for (int w = 0; w < S::U; ++w)
+            load_dwords<S::VD>(vr[t][e][w], vb[t] + (size_t)(e * slot_bytes) + v_off +
+                                                w * 16 * S::VE * S::EB);
+      if (i + NW < hi) pages_of(i + NW, page);
+      __builtin_amdgcn_sched_barrier(0);
+
+      f32x4 acc[S::NS];
+  #pragma unroll
+      for (int t = 0; t < S::NS; ++t) {
+        acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+  #pragma unroll
+        for (int k = 0; k < S::KS; ++k) M::run(acc[t], kf[t][k], qf[k]);
+      }
+      float x[S::NS][4];
+  #pragma unroll
+      for (int t = 0; t < S::NS; ++t)
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) x[t][e] = acc[t][e] * A.scale_log2;
+      if (!all) {  // what a row does not see: no weight; what none sees may hold anything
+  #pragma unroll
+        for (int t = 0; t < S::NS; ++t)
+  #pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = key0 + 16 * t + 4 * g + e;
+            const bool mine = has[t] && key <= p && (key >= first || key < A.sinks);
+            const bool see = has[t] && key <= p_max && (key >= first_min || key < A.sinks);
+            x[t][e] = mine ? x[t][e] : -INFINITY;
+  #pragma unroll
+            for (int w = 0; w < S::U; ++w)
+  #pragma unroll
+              for (int d = 0; d < S::VD; ++d) vr[t][e][w][d] = see ? vr[t][e][w][d] : 0u;
+          }
+      }
+      float mx = m;
+  #pragma unroll
+      for (int t = 0; t < S::NS; ++t)
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, x[t][e]);
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float base = (mx == -INFINITY ? 0.f : mx) - kBias;
+      if (__any(mx > m)) {
+        const float a = exp2f(m - (base + kBias));
+        l *= a;
+  #pragma unroll
+        for (int k = 0; k < S::U * S::VE; ++k) o[k] *= a;
+      }
+      m = mx;
+  #pragma unroll
+      for (int t = 0; t < S::NS; ++t)
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[t][e] = exp2f(x[t][e] - base);
+          l += x[t][e];
+        }
+      Frag pf;
+      if constexpr (DT == DT_F32) {
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) pf.f[e] = x[0][e];
+      } else {
+  #pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          pf.d[2 * t] = pack2<DT>(x[t][0], x[t][1]);
+          pf.d[2 * t + 1] = pack2<DT>(x[t][2], x[t][3]);
+        }
+      }
+  #pragma unroll
+      for (int w = 0; w < S::U; ++w)
+  #pragma unroll
+        for (int f = 0; f < S::VE; ++f) {
+          Frag vf;
+          if constexpr (DT == DT_F32) {
+  #pragma unroll
+            for (int e = 0; e < 4; ++e) vf.f[e] = __uint_as_float(vr[0][e][w][f]);
+          } else {
+  #pragma unroll
+            for (int d = 0; d < 4; ++d) {
+              const uint32_t a = vr[d / 2][2 * (d % 2)][w][f / 2];
+              const uint32_t b = vr[d / 2][2 * (d % 2) + 1][w][f / 2];
+              vf.d[d] = __builtin_amdgcn_perm(b, a, f % 2 ? 0x07060302u : 0x05040100u);
+            }
+          }
+          M::run(o[w * S::VE + f], vf, pf);
+        }
     }
-    const int64_t at = CHUNKS
-                           ? (chunk.t0 + (row_a + k) / G) * A.heads + kh * G + (row_a + k) % G
-                           : (int64_t)s * A.heads + kh * G + row_a + k;
-    if (whole) {
-      acc *= sum == 0.f ? 0.f : 1.f / sum;
-      if constexpr (DT == DT_F32)
-        *(f32x4*)(A.out + (at * HD + d) * 4) = acc;
-      else
-        *(uint2*)(A.out + (at * HD + d) * 2) =
-            uint2{pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3])};
-    } else {
-      *(f32x4*)(A.part_o + ((at * A.n_split + blockIdx.x) * HD + d)) = acc;
-      if (d == 0) {
-        float* ml = A.part_ml + 2 * (at * A.n_split + blockIdx.x);
-        ml[0] = top;
-        ml[1] = sum;
+
+    // join the waves: sums over the lane groups, then o through LDS
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) {
+      sh_m[wave][c] = m;
+      sh_l[wave][c] = l;
+    }
+    if (c < rows) {
+  #pragma unroll
+      for (int w = 0; w < S::U; ++w)
+  #pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float* to = sh_o + (wave * rows + c) * HD + w * 16 * S::VE + (4 * g + e) * S::VE;
+  #pragma unroll
+          for (int f = 0; f < S::VE; f += 4)
+            *(f32x4*)(to + f) = f32x4{o[w * S::VE + f][e], o[w * S::VE + f + 1][e],
+                                      o[w * S::VE + f + 2][e], o[w * S::VE + f + 3][e]};
+        }
+    }
+    __syncthreads();
+    for (int i = threadIdx.x * 4; i < rows * HD; i += NW * 256) {
+      const int k = i / HD, d = i % HD;
+      float top = sh_m[0][k];
+  #pragma unroll
+      for (int w = 1; w < NW; ++w) top = fmaxf(top, sh_m[w][k]);
+      const float base = top == -INFINITY ? 0.f : top;
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.f;
+  #pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float a = exp2f(sh_m[w][k] - base);
+        sum += sh_l[w][k] * a;
+        acc += *(const f32x4*)(sh_o + (w * rows + k) * HD + d) * a;
+      }
+      const int64_t at = CHUNKS
+                             ? (chunk.t0 + (row_a + k) / G) * A.heads + kh * G + (row_a + k) % G
+                             : (int64_t)s * A.heads + kh * G + row_a + k;
+      if (whole) {
+        acc *= sum == 0.f ? 0.f : 1.f / sum;
+        if constexpr (DT == DT_F32)
+          *(f32x4*)(A.out + (at * HD + d) * 4) = acc;
+        else
+          *(uint2*)(A.out + (at * HD + d) * 2) =
+              uint2{pack2<DT>(acc[0], acc[1]), pack2<DT>(acc[2], acc[3])};
+      } else {
+        *(f32x4*)(A.part_o + ((at * A.n_split + blockIdx.x) * HD + d)) = acc;
+        if (d == 0) {
+          float* ml = A.part_ml + 2 * (at * A.n_split + blockIdx.x);
+          ml[0] = top;
+          ml[1] = sum;
+        }
       }
     }
-  }
-  if (!CHUNKS) return;  // n_blocks covers the group
-  __syncthreads();      // the next rows use the same LDS
+    if (!CHUNKS) return;  // n_blocks covers the group
+    __syncthreads();      // the next rows use the same LDS
   }
 }
 
@@ -327,7 +339,8 @@ int launch_waves(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hip
   }
   const dim3 grid((unsigned)A.n_split, (unsigned)(C.kv_heads * n_blocks),
                   (unsigned)(C.seqs + (A.cu ? 1 : 0)));
-  hipLaunchKernelGGL((decode_kernel<DT, HD, NW, CHUNKS>), grid, dim3(NW * 64), lds, st, C, A, n_blocks);
+  hipLaunchKernelGGL((decode_kernel<DT, HD, NW, CHUNKS>), grid, dim3(NW * 64), lds, st, C, A,
+                     n_blocks);
   if (A.n_split > 1) launch_join<DT, HD, Shape<DT, HD>::T, kRows>(C, A, st);
   return SSL_OK;
 }

@@ -15,6 +15,16 @@
 //                in any order both operands share); V is transposed on its way
 //                out of LDS (ds_read_tr16), fp32 values are read as they are.
 //
+// What bounds it: 4096 tokens of one sequence, 16 heads of 128, bf16, take 80 µs,
+// 850 TFLOP/s (a large library product: 1157). A round of two tiles takes a
+// workgroup 3800 cycles, in which a SIMD's two waves hold the matrix unit for 2048
+// and the vector unit for about as long; leaving out the loads, the exponentials,
+// the sums or a product's three quarters saves 9 µs, 5, 3 or 13 each, so no one
+// unit is the bound. (The teams half a round apart, by a second barrier: 3 µs more.
+// Row sums by a two-element dot product of the rounded weights: 0.6 less, not kept.)
+// Beside the rounds a workgroup takes 14000 cycles, 5000 of them for its first
+// tile and q to arrive.
+//
 // K and V go from memory into LDS directly, a tile ahead of its use, two
 // buffers a team, one barrier a tile. LDS rows are permuted in 16-byte chunks by
 // the row, so that fragment reads spread over the banks; the permutation is made
@@ -218,391 +228,408 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   const uint64_t v_base = (uint64_t)(uintptr_t)C.v + kh * C.head_stride * T::EB;
   constexpr float kBias = DT == DT_F16 ? 4.f : 0.f;  // fp16 weights are kept 16-fold
 
-  {
-    const int row_a = tile * T::ROWS, row_b = min(row_a + T::ROWS, chunk.rows) - 1;
-    const int p_min = chunk.p0 + row_a / G, p_max = chunk.p0 + row_b / G;
-    const TileRange range = tile_range<T::KT>(max(p_min, 0), p_max, A.window, A.sinks);
-    const int per = part_tiles(A, range.count);
-    const bool whole = per >= range.count;
-    const int lo = split * per, hi = min(lo + per, range.count);
-    if (lo >= hi && split > 0) return;
-    const int limit = p_max + 1;
-    const int w_first = A.window && p_min + 1 > A.window ? p_min + 1 - A.window : 0;
+  const int row_a = tile * T::ROWS, row_b = min(row_a + T::ROWS, chunk.rows) - 1;
+  const int p_min = chunk.p0 + row_a / G, p_max = chunk.p0 + row_b / G;
+  const TileRange range = tile_range<T::KT>(max(p_min, 0), p_max, A.window, A.sinks);
+  const int per = part_tiles(A, range.count);
+  const bool whole = per >= range.count;
+  const int lo = split * per, hi = min(lo + per, range.count);
+  if (lo >= hi && split > 0) return;
+  const int limit = p_max + 1;
+  const int w_first = A.window && p_min + 1 > A.window ? p_min + 1 - A.window : 0;
 
-    // this wave's rows
-    const int r_a = row_a + w * 32;
-    const bool any = r_a <= row_b;
-    const int r = min(r_a + col, row_b);
-    const int64_t token = chunk.t0 + r / G;
-    const int head = kh * G + r % G;
-    const int p = chunk.p0 + r / G;
-    const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
-    const int wp_min = chunk.p0 + r_a / G, wp_max = chunk.p0 + min(r_a + 31, row_b) / G;
-    const int wfirst_min = A.window && wp_min + 1 > A.window ? wp_min + 1 - A.window : 0;
-    const int wfirst_max = A.window && wp_max + 1 > A.window ? wp_max + 1 - A.window : 0;
+  // this wave's rows
+  const int r_a = row_a + w * 32;
+  const bool any = r_a <= row_b;
+  const int r = min(r_a + col, row_b);
+  const int64_t token = chunk.t0 + r / G;
+  const int head = kh * G + r % G;
+  const int p = chunk.p0 + r / G;
+  const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
+  const int wp_min = chunk.p0 + r_a / G, wp_max = chunk.p0 + min(r_a + 31, row_b) / G;
+  const int wfirst_min = A.window && wp_min + 1 > A.window ? wp_min + 1 - A.window : 0;
+  const int wfirst_max = A.window && wp_max + 1 > A.window ? wp_max + 1 - A.window : 0;
 
-    uint4 qf[T::QS];
-    f32x16 o[T::OT];
+  uint4 qf[T::QS];
+  f32x16 o[T::OT];
 #pragma unroll
-    for (int i = 0; i < T::OT; ++i)
+  for (int i = 0; i < T::OT; ++i)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
-    float m = -INFINITY, l = 0.f;
+    for (int e = 0; e < 16; ++e) o[i][e] = 0.f;
+  float m = -INFINITY, l = 0.f;
 
-    const uint32_t lds0 = lds_addr(lds) + team * 4 * T::BUF;
-    // load lanes: LDS chunk lane % CPR of row lane / CPR of an instruction
-    uint32_t k_off[T::NQ], v_off[T::NQ];
-    int l_row[T::NQ];
+  const uint32_t lds0 = lds_addr(lds) + team * 4 * T::BUF;
+  // load lanes: LDS chunk lane % CPR of row lane / CPR of an instruction
+  uint32_t k_off[T::NQ], v_off[T::NQ];
+  int l_row[T::NQ];
 #pragma unroll
-    for (int q = 0; q < T::NQ; ++q) {
-      const int r16 = (T::IPG >= 4 ? (q * 4 + w) * T::RI : (w & 1) * T::RI) + lane / T::CPR;
-      l_row[q] = r16;
-      k_off[q] = r16 * slot_bytes + ((lane % T::CPR) ^ T::swz_k(r16)) * 16;
-      v_off[q] = r16 * slot_bytes + ((lane % T::CPR) ^ T::swz_v(r16)) * 16;
-    }
-    // page of group lane % (KT / 16) of tile i
-    auto pages_of = [&](int i) {
-      const int key = range.tile(min(i, hi - 1)) * T::KT + 16 * (lane % (T::KT / 16));
-      return table[min(key >> C.log2_page, C.cols - 1)];
-    };
-    // The next tile's loads. Each lane settles one group of 16 positions (group
-    // lane % (KT / 16)): its place in the pools and the bytes of it that are
-    // loaded; load<I> reads them from that lane and issues the wave's I-th loads of
-    // K and V. A tile that does not exist loads zeros.
-    constexpr int KG = T::KT / 16;
-    constexpr int LOADS = (T::IPG >= 4 ? KG : KG / 2) * T::NQ;
-    uint64_t off_l = 0;
-    uint32_t size_l = 0, next_lds = 0, hide_span = 0;
-    int hide_from = 0;
-    auto next_tile = [&](int i, int buf, int32_t page) {
-      const int key0 = range.tile(i) * T::KT;
-      const int key_l = key0 + 16 * (lane % KG);
-      const bool has = C.has(page) && i < hi;
-      off_l = (uint64_t)(uint32_t)(has ? page : 0) * page_bytes +
-              (uint32_t)(key_l & (C.page - 1)) * slot_bytes;
-      size_l = has ? min(max(limit - key_l, 0), 16) * slot_bytes : 0u;
-      next_lds = lds0 + 2 * buf * T::BUF + w * 1024;
-      // positions from sinks to the window's first: zeros as well
-      hide_from = key0 - A.sinks;
-      hide_span = key0 < w_first ? max(w_first - A.sinks, 0) : 0;
-    };
-    auto load = [&](auto at) {
-      constexpr int n = decltype(at)::value / T::NQ, q = decltype(at)::value % T::NQ;
-      const int grp = T::IPG >= 4 ? n : 2 * n + (w >> 1);
-      const uint64_t off =
-          ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off_l >> 32), grp) << 32) |
-          (uint32_t)__builtin_amdgcn_readlane((int)off_l, grp);
-      const uint64_t ka = k_base + off, va = v_base + off;
-      u32x4 rk, rv;
-      rk[0] = (uint32_t)ka;
-      rk[1] = (uint32_t)(ka >> 32);
-      rv[0] = (uint32_t)va;
-      rv[1] = (uint32_t)(va >> 32);
-      rk[2] = rv[2] = __builtin_amdgcn_readlane((int)size_l, grp);
-      rk[3] = rv[3] = 0x00020000u;
-      const uint32_t hide =
-          (uint32_t)(hide_from + 16 * grp + l_row[q]) < hide_span ? 0x80000000u : 0u;
-      // the instruction fills 1 KiB at n · max(IPG, 4) + 4 q + w
-      constexpr int to = (n * (T::IPG >= 4 ? T::IPG : 4) + 4 * q) * 1024;
-      dma16<to>(rk, k_off[q] | hide, next_lds);
-      dma16<to + T::BUF>(rv, v_off[q] | hide, next_lds);
-    };
+  for (int q = 0; q < T::NQ; ++q) {
+    const int r16 = (T::IPG >= 4 ? (q * 4 + w) * T::RI : (w & 1) * T::RI) + lane / T::CPR;
+    l_row[q] = r16;
+    k_off[q] = r16 * slot_bytes + ((lane % T::CPR) ^ T::swz_k(r16)) * 16;
+    v_off[q] = r16 * slot_bytes + ((lane % T::CPR) ^ T::swz_v(r16)) * 16;
+  }
+  // page of group lane % (KT / 16) of tile i
+  auto pages_of = [&](int i) {
+    const int key = range.tile(min(i, hi - 1)) * T::KT + 16 * (lane % (T::KT / 16));
+    return table[min(key >> C.log2_page, C.cols - 1)];
+  };
+  // The next tile's loads. Each lane settles one group of 16 positions (group
+  // lane % (KT / 16)): its place in the pools and the bytes of it that are
+  // loaded; load<I> reads them from that lane and issues the wave's I-th loads of
+  // K and V. A tile that does not exist loads zeros.
+  constexpr int KG = T::KT / 16;
+  constexpr int LOADS = (T::IPG >= 4 ? KG : KG / 2) * T::NQ;
+  uint64_t off_l = 0;
+  uint32_t size_l = 0, next_lds = 0, hide_span = 0;
+  int hide_from = 0;
+  auto next_tile = [&](int i, int buf, int32_t page) {
+    const int key0 = range.tile(i) * T::KT;
+    const int key_l = key0 + 16 * (lane % KG);
+    const bool has = C.has(page) && i < hi;
+    off_l = (uint64_t)(uint32_t)(has ? page : 0) * page_bytes +
+            (uint32_t)(key_l & (C.page - 1)) * slot_bytes;
+    size_l = has ? min(max(limit - key_l, 0), 16) * slot_bytes : 0u;
+    next_lds = lds0 + 2 * buf * T::BUF + w * 1024;
+    // positions from sinks to the window's first: zeros as well
+    hide_from = key0 - A.sinks;
+    hide_span = key0 < w_first ? max(w_first - A.sinks, 0) : 0;
+  };
+  auto load = [&](auto at) {
+    constexpr int n = decltype(at)::value / T::NQ, q = decltype(at)::value % T::NQ;
+    const int grp = T::IPG >= 4 ? n : 2 * n + (w >> 1);
+    const uint64_t off =
+        ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off_l >> 32), grp) << 32) |
+        (uint32_t)__builtin_amdgcn_readlane((int)off_l, grp);
+    const uint64_t ka = k_base + off, va = v_base + off;
+    u32x4 rk, rv;
+    rk[0] = (uint32_t)ka;
+    rk[1] = (uint32_t)(ka >> 32);
+    rv[0] = (uint32_t)va;
+    rv[1] = (uint32_t)(va >> 32);
+    rk[2] = rv[2] = __builtin_amdgcn_readlane((int)size_l, grp);
+    rk[3] = rv[3] = 0x00020000u;
+    const uint32_t hide =
+        (uint32_t)(hide_from + 16 * grp + l_row[q]) < hide_span ? 0x80000000u : 0u;
+    // the instruction fills 1 KiB at n · max(IPG, 4) + 4 q + w
+    constexpr int to = (n * (T::IPG >= 4 ? T::IPG : 4) + 4 * q) * 1024;
+    dma16<to>(rk, k_off[q] | hide, next_lds);
+    dma16<to + T::BUF>(rv, v_off[q] | hide, next_lds);
+  };
 
-    // Fragment addresses in the first buffer: step k of a K row and output tile d
-    // of V differ by an exclusive or below 256 bytes (the permutation's reach) and
-    // by a plain offset above; the buffers' parity is one more bit to flip.
-    constexpr int KX = std::min(T::QS, T::RB >= 256 ? 8 : 4);
-    constexpr int VX = T::F32 ? 1 : std::min(T::OT, 4);
-    uint32_t kx[KX], vx[VX];
+  // Fragment addresses in the first buffer: step k of a K row and output tile d
+  // of V differ by an exclusive or below 256 bytes (the permutation's reach) and
+  // by a plain offset above; the buffers' parity is one more bit to flip.
+  constexpr int KX = std::min(T::QS, T::RB >= 256 ? 8 : 4);
+  constexpr int VX = T::F32 ? 1 : std::min(T::OT, 4);
+  uint32_t kx[KX], vx[VX];
 #pragma unroll
-    for (int k = 0; k < KX; ++k)
-      kx[k] = lds0 + col * T::RB + (((h ^ T::swz_k(col & 15)) * 16) ^ (k * 32));
-    if constexpr (T::F32) {
-      vx[0] = lds0 + T::BUF + 4 * h * T::RB + col * (HD == 64 ? 8 : 16);
-    } else {
-      const int vr = 4 * h + ((lane & 15) >> 2);
+  for (int k = 0; k < KX; ++k)
+    kx[k] = lds0 + col * T::RB + (((h ^ T::swz_k(col & 15)) * 16) ^ (k * 32));
+  if constexpr (T::F32) {
+    vx[0] = lds0 + T::BUF + 4 * h * T::RB + col * (HD == 64 ? 8 : 16);
+  } else {
+    const int vr = 4 * h + ((lane & 15) >> 2);
 #pragma unroll
-      for (int d = 0; d < VX; ++d)
-        vx[d] = lds0 + T::BUF + vr * T::RB + (lane & 3) * 8 +
-                (((((lane >> 4) & 1) * 2) ^ T::swz_v(vr) ^ (4 * d)) * 16);
-    }
-    auto read_k = [&](int f) {  // fragment f = t · QS + k
-      const int t = f / T::QS, k = f % T::QS;
-      return read16(kx[k % KX] + (k / KX) * KX * 32 + t * 32 * T::RB);
-    };
-    auto read_v = [&](int f) {  // fragment f = j · OT + d
-      const int j = f / T::OT, d = f % T::OT;
-      const uint32_t at = vx[d % VX] + (d / VX) * VX * 64 + 16 * j * T::RB;
-      const uint2 a = read_tr(at), b = read_tr(at + 8 * T::RB);
-      return uint4{a.x, a.y, b.x, b.y};
-    };
-    // One tile of the wave's rows. Fragments are read kAhead before their product
-    // and the order is pinned: left alone the compiler reads each right before
-    // its product and waits. Each step of the second product computes the weights
-    // of the next.
-    constexpr int kAhead = 4;
-    auto tile_step = [&](int key0, uint32_t bad, bool all) {
-      constexpr int KF = T::KS * T::QS;
-      f32x16 x[T::KS];
+    for (int d = 0; d < VX; ++d)
+      vx[d] = lds0 + T::BUF + vr * T::RB + (lane & 3) * 8 +
+              (((((lane >> 4) & 1) * 2) ^ T::swz_v(vr) ^ (4 * d)) * 16);
+  }
+  auto read_k = [&](int f) {  // fragment f = t · QS + k
+    const int t = f / T::QS, k = f % T::QS;
+    return read16(kx[k % KX] + (k / KX) * KX * 32 + t * 32 * T::RB);
+  };
+  auto read_v = [&](int f) {  // fragment f = j · OT + d
+    const int j = f / T::OT, d = f % T::OT;
+    const uint32_t at = vx[d % VX] + (d / VX) * VX * 64 + 16 * j * T::RB;
+    const uint2 a = read_tr(at), b = read_tr(at + 8 * T::RB);
+    return uint4{a.x, a.y, b.x, b.y};
+  };
+  // One tile of the wave's rows. Fragments are read kAhead before their product
+  // and the order is pinned: left alone the compiler reads each right before
+  // its product and waits. Each step of the second product computes the weights
+  // of the next.
+  constexpr int kAhead = 4;
+  auto tile_step = [&](int key0, uint32_t bad, bool all) {
+    constexpr int KF = T::KS * T::QS;
+    f32x16 x[T::KS];
 #pragma unroll
-      for (int t = 0; t < T::KS; ++t)
+    for (int t = 0; t < T::KS; ++t)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x[t][e] = 0.f;
-      {
-        uint4 f[kAhead];
+      for (int e = 0; e < 16; ++e) x[t][e] = 0.f;
+    {
+      uint4 f[kAhead];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
+      for (int i = 0; i < kAhead; ++i) f[i] = read_k(i);
+      __builtin_amdgcn_sched_barrier(0);
+      unroll<KF>([&](auto at) {
+        constexpr int i = decltype(at)::value;
+        const uint4 kf = f[i % kAhead], q = qf[i % T::QS];
+        f32x16& acc = x[i / T::QS];
+        if constexpr (T::F32) {
+          mma_f32(acc, __uint_as_float(kf.x), __uint_as_float(q.x));
+          mma_f32(acc, __uint_as_float(kf.y), __uint_as_float(q.y));
+          mma_f32(acc, __uint_as_float(kf.z), __uint_as_float(q.z));
+          mma_f32(acc, __uint_as_float(kf.w), __uint_as_float(q.w));
+        } else {
+          mma<DT>(acc, kf, q);
+        }
+        if constexpr (i + kAhead < KF) f[i % kAhead] = read_k(i + kAhead);
+        if constexpr (i % (KF / LOADS) == 1)
+          load(std::integral_constant<int, i / (KF / LOADS)>{});
         __builtin_amdgcn_sched_barrier(0);
-        unroll<KF>([&](auto at) {
-          constexpr int i = decltype(at)::value;
-          const uint4 kf = f[i % kAhead], q = qf[i % T::QS];
-          f32x16& acc = x[i / T::QS];
-          if constexpr (T::F32) {
-            mma_f32(acc, __uint_as_float(kf.x), __uint_as_float(q.x));
-            mma_f32(acc, __uint_as_float(kf.y), __uint_as_float(q.y));
-            mma_f32(acc, __uint_as_float(kf.z), __uint_as_float(q.z));
-            mma_f32(acc, __uint_as_float(kf.w), __uint_as_float(q.w));
-          } else {
-            mma<DT>(acc, kf, q);
-          }
-          if constexpr (i + kAhead < KF) f[i % kAhead] = read_k(i + kAhead);
-          if constexpr (i % (KF / LOADS) == 1)
-            load(std::integral_constant<int, i / (KF / LOADS)>{});
-          __builtin_amdgcn_sched_barrier(0);
-        });
-      }
-      constexpr int VF = 2 * T::KS * T::OT;
-      uint4 vf[T::F32 ? 1 : kAhead];
-      if constexpr (!T::F32) {
-#pragma unroll
-        for (int i = 0; i < kAhead; ++i) vf[i] = read_v(i);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-      if (!all) {
-#pragma unroll
-        for (int t = 0; t < T::KS; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const int key = key0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
-            const bool see = key <= p && (key >= first || key < A.sinks) &&
-                             !((bad >> (2 * t + (e >> 3))) & 1);
-            x[t][e] = see ? x[t][e] : -INFINITY;
-          }
-      }
-      whole_registers(x);
-      float mx = x[0][0];
-#pragma unroll
-      for (int t = 0; t < T::KS; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
-      {  // with the row's other lane
-        const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
-                                                           false, false);
-        mx = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * A.scale_log2;
-      }
-      // o and l keep an older maximum while it is at most 2^8 too small: the
-      // weights stay in range and most tiles need no scaling
-      if (__any(mx > m + 8.f)) {
-        const float top = fmaxf(m, mx);
-        const float a = exp2f(m - (top == -INFINITY ? 0.f : top));
-        l *= a;
-#pragma unroll
-        for (int d = 0; d < T::OT; ++d)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[d][e] *= a;
-        m = top;
-      }
-      const float base = (m == -INFINITY ? 0.f : m) - kBias;
-      auto weight = [&](int i) {
-        const float y = __builtin_amdgcn_exp2f(fmaf(x[i >> 4][i & 15], A.scale_log2, -base));
-        x[i >> 4][i & 15] = y;
-        l += y;
-      };
-      if constexpr (T::F32) {
-#pragma unroll
-        for (int i = 0; i < 16 * T::KS; ++i) weight(i);
-#pragma unroll
-        for (int t = 0; t < T::KS; ++t)
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            const uint32_t at = vx[0] + (32 * t + 8 * (e >> 2) + (e & 3)) * T::RB;
-            if constexpr (HD == 64) {
-              const uint2 v = read8(at);
-              mma_f32(o[0], __uint_as_float(v.x), x[t][e]);
-              mma_f32(o[1], __uint_as_float(v.y), x[t][e]);
-            } else {
-#pragma unroll
-              for (int d = 0; d < T::OT; d += 4) {
-                const uint4 v = read16(at + d * 128);
-                mma_f32(o[d], __uint_as_float(v.x), x[t][e]);
-                mma_f32(o[d + 1], __uint_as_float(v.y), x[t][e]);
-                mma_f32(o[d + 2], __uint_as_float(v.z), x[t][e]);
-                mma_f32(o[d + 3], __uint_as_float(v.w), x[t][e]);
-              }
-            }
-          }
-      } else {
-        auto packed = [&](int j) {
-          const f32x16& y = x[j >> 1];
-          const int e = 8 * (j & 1);
-          return uint4{pack2<DT>(y[e], y[e + 1]), pack2<DT>(y[e + 2], y[e + 3]),
-                       pack2<DT>(y[e + 4], y[e + 5]), pack2<DT>(y[e + 6], y[e + 7])};
-        };
-#pragma unroll
-        for (int i = 0; i < 8; ++i) weight(i);
-        uint4 pf = packed(0);
-#pragma unroll
-        for (int i = 0; i < VF; ++i) {
-          const int j = i / T::OT, d = i % T::OT;
-          mma<DT>(o[d], vf[i % kAhead], pf);
-          if (i + kAhead < VF) vf[i % kAhead] = read_v(i + kAhead);
-          if (j + 1 < 2 * T::KS) {
-#pragma unroll
-            for (int k = 8 * d / T::OT; k < 8 * (d + 1) / T::OT; ++k) weight(8 * (j + 1) + k);
-            if (d == T::OT - 1) pf = packed(j + 1);
-          }
-          __builtin_amdgcn_sched_barrier(0);
-        }
-      }
-    };
-
-    const int rounds = (hi - lo + T::TEAMS - 1) / T::TEAMS;
-    int32_t pgv = 0;
-    uint32_t bad_next = 0;  // groups of 16 of the tile that lie on no page
-    auto missing = [&](int32_t pg) {
-      return (uint32_t)__ballot(!C.has(pg)) & ((1u << (T::KT / 16)) - 1);
-    };
-    if (rounds > 0) {
-      pgv = pages_of(lo + team);
-      bad_next = missing(pgv);
-      next_tile(lo + team, 0, pgv);
-      unroll<LOADS>(load);
-      pgv = pages_of(lo + team + T::TEAMS);
+      });
     }
-#pragma unroll
-    for (int i = 0; i < T::QS; ++i) {  // after the first tile's loads, to arrive with them
-      qf[i] = *(const uint4*)(A.q + (token * A.q_token + (int64_t)head * A.q_head) * T::EB +
-                              (2 * i + h) * 16);
-      const uint32_t flip = A.flip & (T::F32 ? 0x80000000u : 0x80008000u);
-      qf[i] = uint4{(qf[i].x & A.keep) ^ flip, (qf[i].y & A.keep) ^ flip,
-                    (qf[i].z & A.keep) ^ flip, (qf[i].w & A.keep) ^ flip};
-    }
-    if (!any) {  // a wave without rows only loads
-      for (int n = 0; n < rounds; ++n) {
-        const int i = lo + n * T::TEAMS + team;
-        wait_loads();
-        barrier();
-        next_tile(i + T::TEAMS, (n + 1) & 1, pgv);
-        pgv = pages_of(i + 2 * T::TEAMS);
-        unroll<LOADS>(load);
-      }
-    } else {
-      for (int n = 0; n < rounds; ++n) {
-        const int i = lo + n * T::TEAMS + team;
-        wait_loads();
-        barrier();
-        // a tile past the end, or seen by no row, runs masked: its workgroup waits
-        // for the others' anyway, and a path around it costs copies of o
-        const uint32_t bad = i < hi ? bad_next : ~0u;
-        bad_next = missing(pgv);
-        next_tile(i + T::TEAMS, (n + 1) & 1, pgv);
-        pgv = pages_of(i + 2 * T::TEAMS);
-        const int key0 = range.tile(i) * T::KT;
-        const bool all = key0 + T::KT - 1 <= wp_min && !bad &&
-                         (key0 >= wfirst_max || key0 + T::KT <= A.sinks);
-        tile_step(key0, bad, all);
-#pragma unroll
-        for (int k = 0; k < KX; ++k) kx[k] ^= 2 * T::BUF;  // the other buffers
-#pragma unroll
-        for (int k = 0; k < VX; ++k) vx[k] ^= 2 * T::BUF;
-      }
-    }
-    wait_loads();
-    l += __shfl_xor(l, 32);
-
-    // The teams' parts are joined, each team half of the output tiles: it leaves
-    // the other's half in LDS and takes its own from there.
-    constexpr int HALF = T::OT / T::TEAMS;
-    if constexpr (T::TEAMS == 2) {
-      barrier();
-      f32x4* part = (f32x4*)lds + (w * HALF * 4) * 64 + lane;  // [team][wave][tile][4][lane]
-      float* ml = (float*)(lds + 2 * 4 * HALF * 4 * 64 * 16) + w * 128 + lane;
-      constexpr int STEP = 4 * HALF * 4 * 64;
-#pragma unroll
-      for (int d = 0; d < HALF; ++d)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          f32x4 y;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) y[e] = team ? o[d][4 * k + e] : o[HALF + d][4 * k + e];
-          part[team * STEP + (d * 4 + k) * 64] = y;
-        }
-      ml[team * 512] = m;
-      ml[team * 512 + 64] = l;
-      barrier();
-      const float m2 = ml[(team ^ 1) * 512], l2 = ml[(team ^ 1) * 512 + 64];
-      const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
-      const float a = exp2f(m - base), b = exp2f(m2 - base);
-      // in the order of the teams, so that both halves have one l
-      l = team ? l2 * b + l * a : l * a + l2 * b;
-      m = top;
-#pragma unroll
-      for (int d = 0; d < HALF; ++d)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const f32x4 y = part[(team ^ 1) * STEP + (d * 4 + k) * 64];
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            o[d][4 * k + e] = (team ? o[HALF + d][4 * k + e] : o[d][4 * k + e]) * a + y[e] * b;
-        }
-    }
-    if (r_a + col > row_b) return;
-    const int64_t at = token * A.heads + head;
-    float inv = 1.f;
-    if (whole) {
-      inv = l == 0.f ? 0.f : 1.f / l;
-    } else if (h == 0 && team == 0) {
-      float* ml = A.part_ml + 2 * (at * A.n_split + split);
-      ml[0] = m;
-      ml[1] = l;
-    }
-    // 4 adjacent features at a time, or one
-    auto put1 = [&](int f, float y) {
-      float* to = whole ? (float*)A.out + at * HD : A.part_o + (at * A.n_split + split) * HD;
-      to[f] = y;
-    };
-    auto put = [&](int f, const f32x4 y) {
-      if (!whole)
-        *(f32x4*)(A.part_o + (at * A.n_split + split) * HD + f) = y;
-      else if constexpr (T::F32)
-        *(f32x4*)(A.out + (at * HD + f) * 4) = y;
-      else
-        *(uint2*)(A.out + (at * HD + f) * 2) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
-    };
+    constexpr int VF = 2 * T::KS * T::OT;
+    uint4 vf[T::F32 ? 1 : kAhead];
     if constexpr (!T::F32) {
 #pragma unroll
-      for (int d = 0; d < HALF; ++d)
+      for (int i = 0; i < kAhead; ++i) vf[i] = read_v(i);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!all) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          put(32 * (team * HALF + d) + 8 * k + 4 * h,
-              f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * inv);
-    } else {
-      // fp32: feature f of a lane's vector lies in output tile f, so a team holds
-      // HALF adjacent ones
-      constexpr int VE = std::min(T::OT, 4);
-#pragma unroll
-      for (int d = 0; d < HALF; d += 4)
+      for (int t = 0; t < T::KS; ++t)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
-          const int f = 32 * d + VE * (8 * (e >> 2) + 4 * h + (e & 3)) + team * HALF;
-          if constexpr (HALF >= 4) {
-            put(f, f32x4{o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]} * inv);
-          } else {
-#pragma unroll
-            for (int i = 0; i < HALF; ++i) put1(f + i, o[i][e] * inv);
-          }
+          const int key = key0 + 32 * t + 8 * (e >> 2) + 4 * h + (e & 3);
+          const bool see = key <= p && (key >= first || key < A.sinks) &&
+                           !((bad >> (2 * t + (e >> 3))) & 1);
+          x[t][e] = see ? x[t][e] : -INFINITY;
         }
     }
+    whole_registers(x);
+    float mx = x[0][0];
+#pragma unroll
+    for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mx = fmaxf(mx, x[t][e]);
+    {  // with the row's other lane
+      const auto both = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx),
+                                                         false, false);
+      mx = fmaxf(__uint_as_float(both[0]), __uint_as_float(both[1])) * A.scale_log2;
+    }
+    // o and l keep an older maximum while it is at most 2^8 too small: the
+    // weights stay in range and most tiles need no scaling
+    if (__any(mx > m + 8.f)) {
+      const float top = fmaxf(m, mx);
+      const float a = exp2f(m - (top == -INFINITY ? 0.f : top));
+      l *= a;
+#pragma unroll
+      for (int d = 0; d < T::OT; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[d][e] *= a;
+      m = top;
+    }
+    const float base = (m == -INFINITY ? 0.f : m) - kBias;
+    auto weight = [&](int i) {
+      const float y = __builtin_amdgcn_exp2f(fmaf(x[i >> 4][i & 15], A.scale_log2, -base));
+      x[i >> 4][i & 15] = y;
+      l += y;
+    };
+    if constexpr (T::F32) {
+#pragma unroll
+      for (int i = 0; i < 16 * T::KS; ++i) weight(i);
+#pragma unroll
+      for (int t = 0; t < T::KS; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const uint32_t at = vx[0] + (32 * t + 8 * (e >> 2) + (e & 3)) * T::RB;
+          if constexpr (HD == 64) {
+            const uint2 v = read8(at);
+            mma_f32(o[0], __uint_as_float(v.x), x[t][e]);
+            mma_f32(o[1], __uint_as_float(v.y), x[t][e]);
+          } else {
+#pragma unroll
+            for (int d = 0; d < T::OT; d += 4) {
+              const uint4 v = read16(at + d * 128);
+              mma_f32(o[d], __uint_as_float(v.x), x[t][e]);
+              mma_f32(o[d + 1], __uint_as_float(v.y), x[t][e]);
+              mma_f32(o[d + 2], __uint_as_float(v.z), x[t][e]);
+              mma_f32(o[d + 3], __uint_as_float(v.w), x[t][e]);
+            }
+          }
+        }
+    } else {
+      auto packed = [&](int j) {
+        const f32x16& y = x[j >> 1];
+        const int e = 8 * (j & 1);
+        return uint4{pack2<DT>(y[e], y[e + 1]), pack2<DT>(y[e + 2], y[e + 3]),
+                     pack2<DT>(y[e + 4], y[e + 5]), pack2<DT>(y[e + 6], y[e + 7])};
+      };
+#pragma unroll
+      for (int i = 0; i < 8; ++i) weight(i);
+      uint4 pf = packed(0);
+#pragma unroll
+      for (int i = 0; i < VF; ++i) {
+        const int j = i / T::OT, d = i % T::OT;
+        mma<DT>(o[d], vf[i % kAhead], pf);
+        if (i + kAhead < VF) vf[i % kAhead] = read_v(i + kAhead);
+        if (j + 1 < 2 * T::KS) {
+#pragma unroll
+          for (int k = 8 * d / T::OT; k < 8 * (d + 1) / T::OT; ++k) weight(8 * (j + 1) + k);
+          if (d == T::OT - 1) pf = packed(j + 1);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+
+  const int rounds = (hi - lo + T::TEAMS - 1) / T::TEAMS;
+  int32_t pgv = 0;
+  uint32_t bad_next = 0;  // groups of 16 of the tile that lie on no page
+  auto missing = [&](int32_t pg) {
+    return (uint32_t)__ballot(!C.has(pg)) & ((1u << (T::KT / 16)) - 1);
+  };
+  if (rounds > 0) {
+    pgv = pages_of(lo + team);
+    bad_next = missing(pgv);
+    next_tile(lo + team, 0, pgv);
+    unroll<LOADS>(load);
+    pgv = pages_of(lo + team + T::TEAMS);
+  }
+#pragma unroll
+  for (int i = 0; i < T::QS; ++i) {  // after the first tile's loads, to arrive with them
+    qf[i] = *(const uint4*)(A.q + (token * A.q_token + (int64_t)head * A.q_head) * T::EB +
+                            (2 * i + h) * 16);
+    const uint32_t flip = A.flip & (T::F32 ? 0x80000000u : 0x80008000u);
+    qf[i] = uint4{(qf[i].x & A.keep) ^ flip, (qf[i].y & A.keep) ^ flip,
+                  (qf[i].z & A.keep) ^ flip, (qf[i].w & A.keep) ^ flip};
+  }
+  if (!any) {  // a wave without rows only loads
+    for (int n = 0; n < rounds; ++n) {
+      const int i = lo + n * T::TEAMS + team;
+      wait_loads();
+      barrier();
+      next_tile(i + T::TEAMS, (n + 1) & 1, pgv);
+      pgv = pages_of(i + 2 * T::TEAMS);
+      unroll<LOADS>(load);
+    }
+  } else {
+    for (int n = 0; n < rounds; ++n) {
+      const int i = lo + n * T::TEAMS + team;
+      wait_loads();
+      barrier();
+      // a tile past the end, or seen by no row, runs masked: its workgroup waits
+      // for the others' anyway, and a path around it costs copies of o
+      const uint32_t bad = i < hi ? bad_next : ~0u;
+      bad_next = missing(pgv);
+      next_tile(i + T::TEAMS, (n + 1) & 1, pgv);
+      pgv = pages_of(i + 2 * T::TEAMS);
+      const int key0 = range.tile(i) * T::KT;
+      const bool all = key0 + T::KT - 1 <= wp_min && !bad &&
+                       (key0 >= wfirst_max || key0 + T::KT <= A.sinks);
+      tile_step(key0, bad, all);
+#pragma unroll
+      for (int k = 0; k < KX; ++k) kx[k] ^= 2 * T::BUF;  // the other buffers
+#pragma unroll
+      for (int k = 0; k < VX; ++k) vx[k] ^= 2 * T::BUF;
+    }
+  }
+  wait_loads();
+  l += __shfl_xor(l, 32);
+
+  // The teams' parts are joined, each team half of the output tiles: it leaves
+  // the other's half in LDS and takes its own from there.
+  constexpr int HALF = T::OT / T::TEAMS;
+  if constexpr (T::TEAMS == 2) {
+    barrier();
+    f32x4* part = (f32x4*)lds + (w * HALF * 4) * 64 + lane;  // [team][wave][tile][4][lane]
+    float* ml = (float*)(lds + 2 * 4 * HALF * 4 * 64 * 16) + w * 128 + lane;
+    constexpr int STEP = 4 * HALF * 4 * 64;
+#pragma unroll
+    for (int d = 0; d < HALF; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        f32x4 y;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) y[e] = team ? o[d][4 * k + e] : o[HALF + d][4 * k + e];
+        part[team * STEP + (d * 4 + k) * 64] = y;
+      }
+    ml[team * 512] = m;
+    ml[team * 512 + 64] = l;
+    barrier();
+    const float m2 = ml[(team ^ 1) * 512], l2 = ml[(team ^ 1) * 512 + 64];
+    const float top = fmaxf(m, m2), base = top == -INFINITY ? 0.f : top;
+    const float a = exp2f(m - base), b = exp2f(m2 - base);
+    // in the order of the teams, so that both halves have one l
+    l = team ? l2 * b + l * a : l * a + l2 * b;
+    m = top;
+#pragma unroll
+    for (int d = 0; d < HALF; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const f32x4 y = part[(team ^ 1) * STEP + (d * 4 + k) * 64];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[d][4 * k + e] = (team ? o[HALF + d][4 * k + e] : o[d][4 * k + e]) * a + y[e] * b;
+      }
+  }
+  if (r_a + col > row_b) return;
+  const int64_t at = token * A.heads + head;
+  float inv = 1.f;
+  if (whole) {
+    inv = l == 0.f ? 0.f : 1.f / l;
+  } else if (h == 0 && team == 0) {
+    float* ml = A.part_ml + 2 * (at * A.n_split + split);
+    ml[0] = m;
+    ml[1] = l;
+  }
+  // 4 adjacent features at a time, or one
+  auto put1 = [&](int f, float y) {
+    float* to = whole ? (float*)A.out + at * HD : A.part_o + (at * A.n_split + split) * HD;
+    to[f] = y;
+  };
+  auto put = [&](int f, const f32x4 y) {
+    if (!whole)
+      *(f32x4*)(A.part_o + (at * A.n_split + split) * HD + f) = y;
+    else if constexpr (T::F32)
+      *(f32x4*)(A.out + (at * HD + f) * 4) = y;
+    else
+      *(uint2*)(A.out + (at * HD + f) * 2) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+  };
+  if constexpr (!T::F32) {
+    // 8 adjacent features a lane, its own 4 and the row's other lane's: the stores
+    // of 128 rows 4 KB apart took 4800 cycles of 4 features each, 1.2 µs of 83 at
+    // 4096 tokens
+    if (whole) {
+#pragma unroll
+      for (int d = 0; d < HALF; ++d)
+#pragma unroll
+        for (int k = 0; k < 4; k += 2) {
+          uint32_t y[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            y[i] = pack2<DT>(o[d][4 * k + 2 * i] * inv, o[d][4 * k + 2 * i + 1] * inv);
+          const auto a = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
+          const auto b = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
+          *(uint4*)(A.out + (at * HD + 32 * (team * HALF + d) + 8 * (k + h)) * 2) =
+              uint4{a[0], b[0], a[1], b[1]};
+        }
+      return;
+    }
+#pragma unroll
+    for (int d = 0; d < HALF; ++d)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        put(32 * (team * HALF + d) + 8 * k + 4 * h,
+            f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * inv);
+  } else {
+    // fp32: feature f of a lane's vector lies in output tile f, so a team holds
+    // HALF adjacent ones
+    constexpr int VE = std::min(T::OT, 4);
+#pragma unroll
+    for (int d = 0; d < HALF; d += 4)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int f = 32 * d + VE * (8 * (e >> 2) + 4 * h + (e & 3)) + team * HALF;
+        if constexpr (HALF >= 4) {
+          put(f, f32x4{o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]} * inv);
+        } else {
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) put1(f + i, o[i][e] * inv);
+        }
+      }
   }
 }
 
@@ -619,9 +646,10 @@ int launch(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
     int dev = 0;
     if (int rc = check_hip(hipGetDevice(&dev), "device query")) return rc;
     if (dev < 0 || dev >= 64 || !raised[dev]) {
-      if (int rc = check_hip(hipFuncSetAttribute((const void*)prompt_kernel<DT, HD>,
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS),
-                             "shared memory size"))
+      if (int rc = check_hip(
+              hipFuncSetAttribute((const void*)prompt_kernel<DT, HD>,
+                                  hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS),
+              "shared memory size"))
         return rc;
       if (dev >= 0 && dev < 64) raised[dev] = true;
     }
@@ -642,22 +670,22 @@ int launch_dt(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
 }  // namespace
 
 // Splits contexts where that is faster by an estimate of the launch: a round
-// (a tile a team) takes kRound µs, the rows' workgroups run a device full at a
-// time, and a join costs 4 µs and its parts' traffic at 3 TB/s. (2 prompts of
+// (a tile a team) takes kRound µs with its share of what a workgroup does beside
+// them, the rows' workgroups run a device full at a time, and a join costs 4 µs and its parts' traffic at 3 TB/s. (2 prompts of
 // 1000 tokens, 16 heads of 128: whole 23 µs, in 2 parts 38; 500 tokens, 8 fp32
 // heads of 128: whole 74 µs, in 4 parts 35, in 8 32.) Fills n_split and per;
 // returns the parts' bytes.
 int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
                           int64_t max_length) {
-  // measured rounds, by head_dim 64, 128, 256
+  // by head_dim 64, 128, 256
   static constexpr double kRound[2][3] = {{1.7, 2.2, 2.8}, {3.9, 7.6, 8.9}};
   const bool f32 = dtype == SSL_F32;
   const int KT = f32 ? 32 : 64, G = A->heads / C.kv_heads;
   const int teams = C.head_dim == 256 ? 1 : 2;
   const double slots = (double)device_cus() * (C.head_dim == 64 ? 2 : 1);
   const double round = kRound[f32][C.head_dim == 64 ? 0 : C.head_dim == 128 ? 1 : 2];
-  const int64_t tiles = std::min<int64_t>(C.seqs * std::max<int64_t>(1, (max_tokens * G + 127) / 128),
-                                          A->tokens * G / 128 + C.seqs);
+  const int64_t per_seq = std::max<int64_t>(1, (max_tokens * G + 127) / 128);
+  const int64_t tiles = std::min<int64_t>(C.seqs * per_seq, A->tokens * G / 128 + C.seqs);
   const int64_t blocks = std::max<int64_t>(1, tiles * C.kv_heads);
   int64_t reach = max_length;
   double mean = 1 - 0.5 * max_tokens / std::max<double>(1, max_length);  // of the rows' contexts
