@@ -429,32 +429,37 @@ __global__ __launch_bounds__(256) void fork_copy_kernel(PagedCache C, PagesArgs 
 
 // compact, launch 1 (one workgroup): L, the moves' (from, to) in work[0 .. 2L)
 // behind the map work[2 pages .. 3 pages) of every page to its new number, and
-// the new reference counts. A thread owns `seg` consecutive pages.
+// the new reference counts. A thread owns `seg` consecutive pages; u counts the
+// pages in use below p, so a hole is the (p − u)-th and a page past L the
+// (u − u(L))-th to move.
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(PagedCache C, PagesArgs A) {
+  __shared__ int below;  // u(L)
   const int64_t P = C.pages;
   const int64_t seg = (P + kPlanThreads - 1) / kPlanThreads;
   const int64_t lo = min(threadIdx.x * seg, P), hi = min(lo + seg, P);
   int32_t *from = A.work, *to = A.work + P, *map = A.work + 2 * P;
   int used = 0, L;
   for (int64_t p = lo; p < hi; ++p) used += A.refs[p] > 0;
-  scan_exclusive(used, &L);
-  int holes = 0, movers = 0, total;
-  for (int64_t p = lo; p < hi; ++p) {
-    const bool live = A.refs[p] > 0;
-    holes += !live && p < L;
-    movers += live && p >= L;
+  const int before = scan_exclusive(used, &L);
+  if (L == P && threadIdx.x == 0) below = L;
+  if (lo <= L && L < hi) {
+    int u = before;
+    for (int64_t p = lo; p < L; ++p) u += A.refs[p] > 0;
+    below = u;
   }
-  int h = scan_exclusive(holes, &total), m = scan_exclusive(movers, &total);
+  __syncthreads();
+  int u = before;
   for (int64_t p = lo; p < hi; ++p) {
     const int r = A.refs[p];
     const bool live = r > 0;
     map[p] = (int)p;
-    if (p >= L || !live) A.refs_out[p] = 0;
-    else A.refs_out[p] = r;
-    if (!live && p < L) to[h++] = (int)p;
-    if (live && p >= L) from[m++] = (int)p;
+    A.refs_out[p] = p < L && live ? r : 0;
+    if (!live && p < L) to[p - u] = (int)p;
+    if (live && p >= L) from[u - below] = (int)p;
+    u += live;
   }
   __syncthreads();
+  const int total = L - below;
   for (int i = threadIdx.x; i < total; i += kPlanThreads) {
     map[from[i]] = to[i];
     A.refs_out[to[i]] = A.refs[from[i]];
