@@ -79,6 +79,7 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
   using Frag = typename M::Frag;
   extern __shared__ float sh_o[];  // [NW][rows][HD]
   __shared__ float sh_m[NW][kRows], sh_l[NW][kRows];
+  __shared__ uint32_t sh_anew;  // rows to be taken anew
 
   const int G = A.heads / C.kv_heads;
   const int kh = blockIdx.y / n_blocks;
@@ -279,6 +280,7 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
                                       o[w * S::VE + f + 2][e], o[w * S::VE + f + 3][e]};
         }
     }
+    if (CHUNKS && threadIdx.x == 0) sh_anew = 0;
     __syncthreads();
     for (int i = threadIdx.x * 4; i < rows * HD; i += NW * 256) {
       const int k = i / HD, d = i % HD;
@@ -294,6 +296,8 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
         sum += sh_l[w][k] * a;
         acc += *(const f32x4*)(sh_o + (w * rows + k) * HD + d) * a;
       }
+      if (CHUNKS && !(acc[0] * 0.f + acc[1] * 0.f + acc[2] * 0.f + acc[3] * 0.f == 0.f))
+        atomicOr(&sh_anew, 1u << k);
       const int64_t at = CHUNKS
                              ? (chunk.t0 + (row_a + k) / G) * A.heads + kh * G + (row_a + k) % G
                              : (int64_t)s * A.heads + kh * G + row_a + k;
@@ -313,8 +317,27 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
         }
       }
     }
-    if (!CHUNKS) return;  // n_blocks covers the group
-    __syncthreads();      // the next rows use the same LDS
+    if (!CHUNKS) return;  // n_blocks covers the group, whose rows see the same
+    __syncthreads();
+    for (int k = wave; k < rows; k += NW) {
+      if (!(sh_anew >> k & 1)) continue;
+      float top = sh_m[0][k], sum = 0.f;
+#pragma unroll
+      for (int w = 1; w < NW; ++w) top = fmaxf(top, sh_m[w][k]);
+      const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int w = 0; w < NW; ++w) sum += sh_l[w][k] * exp2f(sh_m[w][k] - base);
+      const int rk = row_a + k;
+      const int64_t tk = chunk.t0 + rk / G;
+      const int hk = kh * G + rk % G;
+      row_anew<DT, HD, S::T>(
+          C, A, s, kh, tk, hk, chunk.p0 + rk / G, range, lo, hi, base - kBias,
+          sum == 0.f ? 0.f : 1.f / sum,
+          whole ? nullptr : A.part_o + ((tk * A.heads + hk) * A.n_split + blockIdx.x) * HD,
+          [](int) { return true; });
+    }
+    if ((block + n_blocks) * kRows >= n_rows) return;
+    __syncthreads();  // the next rows use the same LDS
   }
 }
 

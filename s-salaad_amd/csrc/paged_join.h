@@ -1,5 +1,6 @@
-// The parts of split contexts joined: a row's parts hold their maximum m, sum l
-// and output o relative to m; the row is Σ o·2^(m − max) / Σ l·2^(m − max).
+// What the two attention kernels share: rows taken anew, and the parts of split
+// contexts joined: a row's parts hold their maximum m, sum l and output o relative
+// to m; the row is Σ o·2^(m − max) / Σ l·2^(m − max).
 #pragma once
 
 #include "paged.h"
@@ -31,6 +32,60 @@ __device__ __forceinline__ int row_parts(const PagedCache& C, const AttnArgs& A,
                                         A.window, A.sinks);
   const int per = part_tiles(A, range.count);
   return per >= range.count ? 0 : (range.count + per - 1) / per;  // one part wrote the output
+}
+
+// The tiles' products give a masked position the weight 0, which takes a NaN or an
+// infinity among its values into the row all the same. A row whose output is not
+// finite is therefore taken anew over tiles lo … hi − 1, by a wave, from the
+// positions that it sees alone, with the maximum (`base`) and sum that it has: the
+// scores of masked positions never entered those. Slow, and for such rows only.
+// part: where the row's part goes, or null for the output; mine(f): the features to
+// write.
+template <int DT, int HD, int T, typename F>
+__device__ __forceinline__ void row_anew(const PagedCache& C, const AttnArgs& A, int s, int kh,
+                                         int64_t token, int head, int p, const TileRange& range,
+                                         int lo, int hi, float base, float inv, float* part,
+                                         F mine) {
+  constexpr int N = HD / 64, EB = Elem<DT>::bytes;
+  const int f0 = (threadIdx.x & 63) * N;
+  const char* q = A.q + (token * A.q_token + (int64_t)head * A.q_head) * EB;
+  const int32_t* row = C.table + (int64_t)s * C.table_stride;
+  const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
+  float qf[N], o[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float x = load_scalar<DT>(q, f0 + i);
+    qf[i] = !A.keep ? 0.f : A.flip ? -x : x;
+    o[i] = 0.f;
+  }
+  for (int key = range.tile(lo) * T, i = lo; i < hi; ++key) {
+    if (key == (range.tile(i) + 1) * T) {
+      if (++i == hi) break;
+      key = range.tile(i) * T;
+    }
+    if (key > p || (key < first && key >= A.sinks)) continue;
+    const int32_t page = row[min(key >> C.log2_page, C.cols - 1)];
+    if (!C.has(page)) continue;
+    const int64_t off = page * C.page_stride + kh * C.head_stride +
+                        (key & (C.page - 1)) * C.slot_stride + f0;
+    float x = 0.f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x = fmaf(qf[j], load_scalar<DT>(C.k, off + j), x);
+#pragma unroll
+    for (int j = 1; j < 64; j <<= 1) x += __shfl_xor(x, j);
+    const float w = exp2f(fmaf(x, A.scale_log2, -base));
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] = fmaf(w, load_scalar<DT>(C.v, off + j), o[j]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int f = f0 + i;
+    if (!mine(f)) continue;
+    const int64_t at = (token * A.heads + head) * HD + f;
+    if (part) part[f] = o[i];
+    else if constexpr (DT == DT_F32) ((float*)A.out)[at] = o[i] * inv;
+    else ((uint16_t*)A.out)[at] = (uint16_t)to_bits<DT>(o[i] * inv);
+  }
 }
 
 // TPR threads a row: HD / 4 lanes take the features, the lane groups every

@@ -565,71 +565,94 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
           o[d][4 * k + e] = (team ? o[HALF + d][4 * k + e] : o[d][4 * k + e]) * a + y[e] * b;
       }
   }
-  if (r_a + col > row_b) return;
   const int64_t at = token * A.heads + head;
-  float inv = 1.f;
-  if (whole) {
-    inv = l == 0.f ? 0.f : 1.f / l;
-  } else if (h == 0 && team == 0) {
-    float* ml = A.part_ml + 2 * (at * A.n_split + split);
-    ml[0] = m;
-    ml[1] = l;
-  }
-  // 4 adjacent features at a time, or one
-  auto put1 = [&](int f, float y) {
-    float* to = whole ? (float*)A.out + at * HD : A.part_o + (at * A.n_split + split) * HD;
-    to[f] = y;
-  };
-  auto put = [&](int f, const f32x4 y) {
-    if (!whole)
-      *(f32x4*)(A.part_o + (at * A.n_split + split) * HD + f) = y;
-    else if constexpr (T::F32)
-      *(f32x4*)(A.out + (at * HD + f) * 4) = y;
-    else
-      *(uint2*)(A.out + (at * HD + f) * 2) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
-  };
-  if constexpr (!T::F32) {
-    // 8 adjacent features a lane, its own 4 and the row's other lane's: the stores
-    // of 128 rows 4 KB apart took 4800 cycles of 4 features each, 1.2 µs of 83 at
-    // 4096 tokens
-    if (whole) {
-#pragma unroll
-      for (int d = 0; d < HALF; ++d)
-#pragma unroll
-        for (int k = 0; k < 4; k += 2) {
-          uint32_t y[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            y[i] = pack2<DT>(o[d][4 * k + 2 * i] * inv, o[d][4 * k + 2 * i + 1] * inv);
-          const auto a = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
-          const auto b = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
-          *(uint4*)(A.out + (at * HD + 32 * (team * HALF + d) + 8 * (k + h)) * 2) =
-              uint4{a[0], b[0], a[1], b[1]};
-        }
-      return;
+  const float inv = !whole ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  if (r_a + col <= row_b) {
+    if (!whole && h == 0 && team == 0) {
+      float* ml = A.part_ml + 2 * (at * A.n_split + split);
+      ml[0] = m;
+      ml[1] = l;
     }
+    // 4 adjacent features at a time, or one
+    auto put1 = [&](int f, float y) {
+      float* to = whole ? (float*)A.out + at * HD : A.part_o + (at * A.n_split + split) * HD;
+      to[f] = y;
+    };
+    auto put = [&](int f, const f32x4 y) {
+      if (!whole)
+        *(f32x4*)(A.part_o + (at * A.n_split + split) * HD + f) = y;
+      else if constexpr (T::F32)
+        *(f32x4*)(A.out + (at * HD + f) * 4) = y;
+      else
+        *(uint2*)(A.out + (at * HD + f) * 2) = uint2{pack2<DT>(y[0], y[1]), pack2<DT>(y[2], y[3])};
+    };
+    if constexpr (!T::F32) {
+      // 8 adjacent features a lane, its own 4 and the row's other lane's: the stores
+      // of 128 rows 4 KB apart took 4800 cycles of 4 features each, 1.2 µs of 83 at
+      // 4096 tokens
+      if (whole) {
 #pragma unroll
-    for (int d = 0; d < HALF; ++d)
+        for (int d = 0; d < HALF; ++d)
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        put(32 * (team * HALF + d) + 8 * k + 4 * h,
-            f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * inv);
-  } else {
-    // fp32: feature f of a lane's vector lies in output tile f, so a team holds
-    // HALF adjacent ones
-    constexpr int VE = std::min(T::OT, 4);
+          for (int k = 0; k < 4; k += 2) {
+            uint32_t y[4];
 #pragma unroll
-    for (int d = 0; d < HALF; d += 4)
+            for (int i = 0; i < 4; ++i)
+              y[i] = pack2<DT>(o[d][4 * k + 2 * i] * inv, o[d][4 * k + 2 * i + 1] * inv);
+            const auto a = __builtin_amdgcn_permlane32_swap(y[0], y[2], false, false);
+            const auto b = __builtin_amdgcn_permlane32_swap(y[1], y[3], false, false);
+            *(uint4*)(A.out + (at * HD + 32 * (team * HALF + d) + 8 * (k + h)) * 2) =
+                uint4{a[0], b[0], a[1], b[1]};
+          }
+      } else {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int f = 32 * d + VE * (8 * (e >> 2) + 4 * h + (e & 3)) + team * HALF;
-        if constexpr (HALF >= 4) {
-          put(f, f32x4{o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]} * inv);
-        } else {
+        for (int d = 0; d < HALF; ++d)
 #pragma unroll
-          for (int i = 0; i < HALF; ++i) put1(f + i, o[i][e] * inv);
-        }
+          for (int k = 0; k < 4; ++k)
+            put(32 * (team * HALF + d) + 8 * k + 4 * h,
+                f32x4{o[d][4 * k], o[d][4 * k + 1], o[d][4 * k + 2], o[d][4 * k + 3]} * inv);
       }
+    } else {
+      // fp32: feature f of a lane's vector lies in output tile f, so a team holds
+      // HALF adjacent ones
+      constexpr int VE = std::min(T::OT, 4);
+#pragma unroll
+      for (int d = 0; d < HALF; d += 4)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int f = 32 * d + VE * (8 * (e >> 2) + 4 * h + (e & 3)) + team * HALF;
+          if constexpr (HALF >= 4) {
+            put(f, f32x4{o[d][e], o[d + 1][e], o[d + 2][e], o[d + 3][e]} * inv);
+          } else {
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) put1(f + i, o[i][e] * inv);
+          }
+        }
+    }
+  }
+
+  float finite = 0.f;
+#pragma unroll
+  for (int d = 0; d < HALF; ++d)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) finite = fmaf(o[d][e], 0.f, finite);
+  const uint64_t lanes = __ballot(r_a + col <= row_b && finite != 0.f);
+  uint32_t anew = (uint32_t)(lanes | lanes >> 32);
+  if (!anew) return;
+  wait_loads();  // and the stores above
+  for (; anew; anew &= anew - 1) {
+    const int c = __builtin_ctz(anew), rc = r_a + c;
+    const int64_t tc = chunk.t0 + rc / G;
+    const int hc = kh * G + rc % G;
+    const float mc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), c));
+    const float ic = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(inv), c));
+    row_anew<DT, HD, T::KT>(
+        C, A, s, kh, tc, hc, chunk.p0 + rc / G, range, lo, hi,
+        (mc == -INFINITY ? 0.f : mc) - kBias, ic,
+        whole ? nullptr : A.part_o + ((tc * A.heads + hc) * A.n_split + split) * HD,
+        [&](int f) {  // the team's own
+          return T::TEAMS == 1 || (T::F32 ? f / HALF % 2 : f / (HD / 2)) == team;
+        });
   }
 }
 

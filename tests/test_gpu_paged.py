@@ -174,6 +174,43 @@ def test_missing_pages_are_not_seen(gpu_device):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("heads,kv,counts,lens,window,sinks,bad", [
+    (2, 1, [70], [70], 0, 0, [40, 69]),              # one row tile of each kernel
+    (2, 1, [600], [600], 0, 0, [3, 300, 599]),       # many
+    (4, 2, [9, 1], [2000, 300], 0, 0, [1995, 299]),  # few rows, contexts in parts
+    (6, 2, [150, 40], [500, 900], 100, 3, [420, 870]),
+    (1, 1, [330], [1200], 0, 0, [1000, 1190])])
+def test_a_chunks_rows_see_no_later_infinity(dt, hd, heads, kv, counts, lens, window, sinks, bad,
+                                             gpu_device):
+    """NaN and infinities among the values of a chunk's later tokens, and before its
+    later tokens' windows: rows that do not see them stay as they are."""
+    import ssalaad_amd as sa
+
+    g = torch.Generator().manual_seed(8)
+    dtype = DT[dt]
+    table, pages = pc.pages_of(lens, 16, g)
+    kp, vp = pc.cache(pages, kv, 16, hd, dtype, g)
+    for s, n in enumerate(lens):
+        for j in bad:
+            if j < n:
+                at = vp[table[s, j // 16], 0, j % 16]
+                at[3], at[hd // 2 + 1], at[hd - 1] = float("nan"), -float("inf"), float("inf")
+    q = torch.randn(sum(counts), heads, hd, generator=g).to(dtype)
+    owners, pos = pc.chunk_rows(counts, lens)
+    want, tol = pc.attention(q, kp, vp, table, owners, pos, 16, window, sinks, None, lens)
+    cu = torch.tensor([0] + counts).cumsum(0).int()
+    d = [t.to(gpu_device) for t in (q, kp, vp, table, torch.tensor(lens, dtype=torch.int32), cu)]
+    got = sa.paged_prompt_attention(*d, window=window, sinks=sinks, max_tokens=max(counts),
+                                    max_length=max(lens)).double().cpu()
+    fine = torch.isfinite(want)
+    assert fine.any() and not fine.all()
+    assert torch.equal(torch.isfinite(got), fine) and torch.equal(got.isnan(), want.isnan())
+    assert ((got - want).abs() <= tol)[fine].all()
+    assert torch.equal(got[~fine].sign().nan_to_num(), want[~fine].sign().nan_to_num())
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 def test_attention_extreme_scores(dt, gpu_device):
     """Scores far apart and all far below zero: the running maximum carries them."""
     import ssalaad_amd as sa
