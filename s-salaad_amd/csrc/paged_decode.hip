@@ -319,8 +319,9 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
     }
     if (!CHUNKS) return;  // n_blocks covers the group, whose rows see the same
     __syncthreads();
-    for (int k = wave; k < rows; k += NW) {
-      if (!(sh_anew >> k & 1)) continue;
+    const uint32_t anew = __builtin_amdgcn_readfirstlane(sh_anew);
+    for (int k = anew ? wave : rows; k < rows; k += NW) {
+      if (!(anew >> k & 1)) continue;
       float top = sh_m[0][k], sum = 0.f;
 #pragma unroll
       for (int w = 1; w < NW; ++w) top = fmaxf(top, sh_m[w][k]);
