@@ -296,7 +296,9 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
         sum += sh_l[w][k] * a;
         acc += *(const f32x4*)(sh_o + (w * rows + k) * HD + d) * a;
       }
-      if (CHUNKS && !(acc[0] * 0.f + acc[1] * 0.f + acc[2] * 0.f + acc[3] * 0.f == 0.f))
+      // (a row whose sum is NaN is NaN by its own scores)
+      if (CHUNKS && sum == sum &&
+          !(acc[0] * 0.f + acc[1] * 0.f + acc[2] * 0.f + acc[3] * 0.f == 0.f))
         atomicOr(&sh_anew, 1u << k);
       const int64_t at = CHUNKS
                              ? (chunk.t0 + (row_a + k) / G) * A.heads + kh * G + (row_a + k) % G

@@ -38,7 +38,8 @@ __device__ __forceinline__ int row_parts(const PagedCache& C, const AttnArgs& A,
 // infinity among its values into the row all the same. A row whose output is not
 // finite is therefore taken anew over tiles lo … hi − 1, by a wave, from the
 // positions that it sees alone, with the maximum (`base`) and sum that it has: the
-// scores of masked positions never entered those. Slow, and for such rows only.
+// scores of masked positions never entered those. (600 tokens of 2 heads of 128, all
+// values NaN: 640 µs, finite 21; 4096 tokens of 16 heads 22 ms, 90 µs.)
 // part: where the row's part goes, or null for the output; mine(f): the features to
 // write.
 template <int DT, int HD, int T, typename F>
@@ -47,35 +48,45 @@ __device__ __forceinline__ void row_anew(const PagedCache& C, const AttnArgs& A,
                                          int lo, int hi, float base, float inv, float* part,
                                          F mine) {
   constexpr int N = HD / 64, EB = Elem<DT>::bytes;
-  const int f0 = (threadIdx.x & 63) * N;
+  const int lane = threadIdx.x & 63, f0 = lane * N;
   const char* q = A.q + (token * A.q_token + (int64_t)head * A.q_head) * EB;
   const int32_t* row = C.table + (int64_t)s * C.table_stride;
   const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
-  float qf[N], o[N];
+  const float sign = A.flip ? -A.scale_log2 : A.scale_log2;
+  float o[N];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const float x = load_scalar<DT>(q, f0 + i);
-    qf[i] = !A.keep ? 0.f : A.flip ? -x : x;
-    o[i] = 0.f;
-  }
-  for (int key = range.tile(lo) * T, i = lo; i < hi; ++key) {
-    if (key == (range.tile(i) + 1) * T) {
-      if (++i == hi) break;
-      key = range.tile(i) * T;
-    }
-    if (key > p || (key < first && key >= A.sinks)) continue;
-    const int32_t page = row[min(key >> C.log2_page, C.cols - 1)];
-    if (!C.has(page)) continue;
-    const int64_t off = page * C.page_stride + kh * C.head_stride +
-                        (key & (C.page - 1)) * C.slot_stride + f0;
+  for (int i = 0; i < N; ++i) o[i] = 0.f;
+  for (int i = lo; i < hi; ++i) {
+    // scores: a lane a position
+    const int key = range.tile(i) * T + lane;
+    bool see = lane < T && key <= p && (key >= first || key < A.sinks);
+    const int32_t page = see ? row[min(key >> C.log2_page, C.cols - 1)] : -1;
+    see = see && C.has(page);
+    const int64_t off = (see ? page * C.page_stride + (key & (C.page - 1)) * C.slot_stride : 0) +
+                        kh * C.head_stride;
     float x = 0.f;
+#pragma unroll 1  // the kernels' registers are for their own loops
+    for (int j = 0; j < HD; j += 16 / EB) {
+      const uint4 a = *(const uint4*)(q + j * EB), b = *(const uint4*)(C.k + (off + j) * EB);
 #pragma unroll
-    for (int j = 0; j < N; ++j) x = fmaf(qf[j], load_scalar<DT>(C.k, off + j), x);
+      for (int e = 0; e < 16 / EB; ++e)
+        x = fmaf(A.keep ? load_scalar<DT>(&a, e) : 0.f, load_scalar<DT>(&b, e), x);
+    }
+    const float w = see ? exp2f(fmaf(x, sign, -base)) : 0.f;
+    // values: a lane N features; a position not seen reads page 0 and counts as zero
+    const uint64_t seen = __ballot(see);
+    if (!seen) continue;
+#pragma unroll 4
+    for (int c = 0; c < T; ++c) {
+      const float wc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(w), c));
+      const int64_t at = ((int64_t)__builtin_amdgcn_readlane((int)(off >> 32), c) << 32) |
+                         (uint32_t)__builtin_amdgcn_readlane((int)off, c);
 #pragma unroll
-    for (int j = 1; j < 64; j <<= 1) x += __shfl_xor(x, j);
-    const float w = exp2f(fmaf(x, A.scale_log2, -base));
-#pragma unroll
-    for (int j = 0; j < N; ++j) o[j] = fmaf(w, load_scalar<DT>(C.v, off + j), o[j]);
+      for (int j = 0; j < N; ++j) {
+        const float v = load_scalar<DT>(C.v, at + f0 + j);
+        o[j] = fmaf(wc, seen >> c & 1 ? v : 0.f, o[j]);
+      }
+    }
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) {

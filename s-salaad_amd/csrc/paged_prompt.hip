@@ -636,7 +636,8 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   for (int d = 0; d < HALF; ++d)
 #pragma unroll
     for (int e = 0; e < 16; ++e) finite = fmaf(o[d][e], 0.f, finite);
-  const uint64_t lanes = __ballot(r_a + col <= row_b && finite != 0.f);
+  // (a row whose sum is NaN is NaN by its own scores)
+  const uint64_t lanes = __ballot(r_a + col <= row_b && finite != 0.f && l == l);
   uint32_t anew = (uint32_t)(lanes | lanes >> 32);
   if (!anew) return;
   wait_loads();  // and the stores above
