@@ -454,18 +454,13 @@ _PLAIN = {"append": _plain_append, "decode": _plain_decode, "prompt": _plain_pro
 
 
 # --------------------------------------------------- the package's own calls --
-_PACKAGE = None
-
-
 def _package():
-    """The package, imported once as a user's program does."""
-    global _PACKAGE
-    if _PACKAGE is None:
-        sys.path.insert(0, str(Path(__file__).resolve().parent.parent / "s-salaad_amd"))
-        import ssalaad_amd
+    at = str(Path(__file__).resolve().parent.parent / "s-salaad_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    import ssalaad_amd
 
-        _PACKAGE = ssalaad_amd
-    return _PACKAGE
+    return ssalaad_amd
 
 
 def _own(s):
