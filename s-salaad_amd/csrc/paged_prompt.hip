@@ -74,10 +74,12 @@ struct Tile {
 
 // 16 bytes a lane from memory into LDS (lane l: lds + OFF + 16·l), zeros past the
 // resource's size. In assembly, so that the compiler adds no waits of its own
-// for it: wait_loads and the barrier below order it.
+// for it: wait_loads and the barrier below order it. (s_nop: the load takes m0 one wait
+// state after a scalar write and its resource five after a vector one, which the
+// compiler cannot see to here; with one state or four the times are the same.)
 template <int OFF>
 __device__ __forceinline__ void dma16(const u32x4& r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_add_u32 m0, %0, %3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+  asm volatile("s_add_u32 m0, %0, %3\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
                : "s"(lds), "v"(voff), "s"(r), "n"(OFF)
                : "m0", "scc");

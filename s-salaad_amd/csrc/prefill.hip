@@ -237,9 +237,11 @@ __device__ __forceinline__ u32x4 rsrc_words(const void* base, int64_t bytes) {
 // (every load of the loop is unconditional, so the counts are exact) and
 // orders LDS access with explicit barriers. No memory clobber: the waits and
 // barriers that order LDS access around these loads are compiler barriers
-// themselves.
+// themselves. s_nop: the load takes m0 one wait state after a scalar write
+// and its resource five after a vector instruction's, which the compiler cannot
+// see to inside the assembly; with one state or four the times are the same.
 __device__ __forceinline__ void dma16(const u32x4& r, uint32_t voff, uint32_t soff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                :
                : "s"(lds), "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff))
                : "m0");
@@ -249,7 +251,7 @@ __device__ __forceinline__ void dma16(const u32x4& r, uint32_t voff, uint32_t so
 // hide.
 __device__ __forceinline__ void dma16_sc1(const u32x4& r, uint32_t voff, uint32_t soff,
                                           uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dwordx4 %1, %2, %3 offen sc1 lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, %3 offen sc1 lds"
                :
                : "s"(lds), "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff))
                : "m0");
@@ -257,7 +259,7 @@ __device__ __forceinline__ void dma16_sc1(const u32x4& r, uint32_t voff, uint32_
 
 // 4 bytes a lane: lane l writes LDS byte address lds + 4·l (active lanes only).
 __device__ __forceinline__ void dma4(const u32x4& r, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds"
                :
                : "s"(lds), "v"(voff), "s"(r)
                : "m0");
