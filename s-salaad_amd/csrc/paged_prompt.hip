@@ -662,8 +662,10 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
 template <int DT, int HD>
 int launch(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
   using T = Tile<DT, HD>;
-  // row tiles at most: a partly filled one a sequence
-  const int64_t n_tiles = A.tokens * (A.heads / C.kv_heads) / T::ROWS + C.seqs;
+  // row tiles at most: a partly filled one a sequence. (None without sequences, of
+  // which a tile's workgroup reads lengths: only the tokens past the last chunk.)
+  const int64_t n_tiles =
+      C.seqs ? A.tokens * (A.heads / C.kv_heads) / T::ROWS + C.seqs : 0;
   const int64_t grid = (n_tiles + 1) * A.n_split * C.kv_heads;
   if (grid > 0x7fffffff)
     return fail(SSL_ERR_UNSUPPORTED, "paged_attention: a grid of %lld workgroups", (long long)grid);

@@ -152,6 +152,19 @@ def test_prompt_rows_that_see_nothing_and_tokens_past_the_last(gpu_device):
         assert (out[:2] == 0).all() and (out[45:] == 0).all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("tokens", [1, 10, 100, 600])  # few rows of a head, and many
+def test_tokens_without_sequences_are_zeros(dt, tokens, gpu_device):
+    import ssalaad_amd as sa
+
+    dev = gpu_device
+    i32 = lambda *s: torch.zeros(*s, dtype=torch.int32, device=dev)  # noqa: E731
+    pool = torch.ones(3, 1, 16, 64, dtype=DT[dt], device=dev)
+    q = torch.ones(tokens, 8, 64, dtype=DT[dt], device=dev)
+    out = sa.paged_prompt_attention(q, pool, pool, i32(0, 4), i32(0), i32(1))
+    assert out.shape == q.shape and not out.any()
+
+
 def test_missing_pages_are_not_seen(gpu_device):
     import ssalaad_amd as sa
 
