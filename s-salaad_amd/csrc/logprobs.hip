@@ -44,11 +44,12 @@ struct LogprobArgs {
   float* top_logprobs;
 };
 
-// NaN counts as the largest; −0 equals +0.
+// NaN counts as the largest, below a key of all ones, which stands for none; −0
+// equals +0.
 __device__ __forceinline__ uint64_t key_of(float x, int i) {
   const uint32_t u = __float_as_uint(x + 0.f);
   uint32_t o = u & 0x80000000u ? ~u : u | 0x80000000u;
-  if (x != x) o = 0xffffffffu;
+  if (x != x) o = 0xfffffffeu;
   return ((uint64_t)o << 32) | (0xffffffffu - (uint32_t)i);
 }
 

@@ -672,6 +672,27 @@ def test_logprobs_of_broken_rows(gpu_device):
         assert got.entropy[3:].isfinite().all() and got.top_logprobs[3:].isfinite().all()
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("vocab,top", [(1, 1), (5, 5), (64, 64), (700, 20)])
+def test_logprobs_order_a_row_of_nans(dt, vocab, top, gpu_device):
+    """NaN first, also in the first place, each index once, the whole row asked for."""
+    import ssalaad_amd as sa
+
+    x = torch.randn(4, vocab, generator=torch.Generator().manual_seed(vocab))
+    x[0, 0] = float("nan")
+    x[1, ::2] = float("nan")
+    x[2] = float("nan")
+    x[3, 0], x[3, -1] = float("inf"), float("nan")
+    x = x.to(DT[dt])
+    order = torch.where(x.isnan(), float("inf"), x.double().clamp(max=1e300))
+    want = torch.sort(order, dim=-1, descending=True, stable=True).indices[:, :top]
+    got = sa.token_logprobs(x.to(gpu_device), torch.zeros(4, dtype=torch.int64, device=gpu_device),
+                            top=top)
+    assert torch.equal(got.top_ids.cpu(), want)
+    assert got.logprobs.isnan().all() and got.entropy.isnan().all()
+    assert got.top_logprobs.isnan().all()
+
+
 def test_logprobs_keep_the_digits_of_a_certain_token(gpu_device):
     """One token with almost all the mass: log p near zero, to fp32 relative accuracy."""
     import ssalaad_amd as sa
