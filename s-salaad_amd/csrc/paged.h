@@ -36,7 +36,7 @@ struct AttnArgs {
   const int32_t *lengths, *cu;
   int64_t tokens;
   int heads, window, sinks;
-  // |scale| · log2 e (scores are kept in base 2; 1 for a scale of 0), and what
+  // |scale| · log2 e (scores are kept in base 2; 1 for a scale whose float is 0), and what
   // its sign does to q: kept bits, flipped sign bits
   float scale_log2;
   uint32_t keep, flip;

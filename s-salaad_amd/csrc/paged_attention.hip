@@ -75,8 +75,10 @@ int attention_args(const ssl_paged_attention_args* a, PagedCache* C, AttnArgs* A
   A->sinks = (int)std::min<int64_t>(a->sinks, 0x7fffffff);
   if (!(fabs(a->scale) < 1e30))
     return fail(SSL_ERR_INVALID, "%s: scale %g", what, a->scale);
-  A->scale_log2 = a->scale == 0 ? 1.f : (float)(fabs(a->scale) * 1.4426950408889634);
-  A->keep = a->scale == 0 ? 0u : ~0u;
+  // (a scale whose float is 0 is one of 0, not a product of it with a masked −inf)
+  const float scale = (float)(fabs(a->scale) * 1.4426950408889634);
+  A->scale_log2 = scale == 0 ? 1.f : scale;
+  A->keep = scale == 0 ? 0u : ~0u;
   A->flip = a->scale < 0 ? ~0u : 0u;
   const int64_t reach = std::min<int64_t>(a->max_length, (int64_t)C->cols * C->page);
   if (C->cols == 0) return fail(SSL_ERR_INVALID, "%s: a table without columns", what);

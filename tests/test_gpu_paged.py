@@ -244,6 +244,16 @@ def test_attention_extreme_scores(dt, gpu_device):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale", [0.0, 1e-44, 1e-46, -1e-46, 5e-324])
+def test_attention_of_a_vanishing_scale(dt, scale, gpu_device):
+    """Means of what is seen, in every kernel: few rows, many, one token each."""
+    _attend(gpu_device, DT[dt], 4, 2, 64, 16, [300, 1, 0], scale=scale)
+    _attend(gpu_device, DT[dt], 4, 2, 64, 16, [90, 30], counts=[40, 30], scale=scale)
+    _attend(gpu_device, DT[dt], 8, 1, 64, 16, [700], counts=[560 if dt == "f32" else 100],
+            window=50, sinks=3, scale=scale)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 def test_attention_strides(dt, gpu_device):
     """q as a view of a fused projection, pools interleaved, a wider table."""
     import ssalaad_amd as sa
