@@ -124,6 +124,16 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// A product rounded before it is used (and not fused into what uses it).
+__device__ __forceinline__ float rounded(float x) {
+  asm("" : "+v"(x));
+  return x;
+}
+// From here on the prompt kernel's weights take rounded scores. (Below, a fused
+// product minus the rounded maximum is off by at most 2^-4 in the exponent, for all
+// of a row alike; above, a half step of the maximum would overflow the weights.)
+constexpr float kFarScore = 1048576.f;
+
 // Few rows of a key/value head (paged_decode.hip), or many (paged_prompt.hip).
 // The plans fill the split and return the bytes of the parts.
 int64_t paged_decode_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,

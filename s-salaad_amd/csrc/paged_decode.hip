@@ -192,7 +192,7 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
   #pragma unroll
       for (int t = 0; t < S::NS; ++t)
   #pragma unroll
-        for (int e = 0; e < 4; ++e) x[t][e] = acc[t][e] * A.scale_log2;
+        for (int e = 0; e < 4; ++e) x[t][e] = rounded(acc[t][e] * A.scale_log2);
       if (!all) {  // what a row does not see: no weight; what none sees may hold anything
   #pragma unroll
         for (int t = 0; t < S::NS; ++t)
@@ -215,9 +215,9 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, x[t][e]);
       mx = fmaxf(mx, __shfl_xor(mx, 16));
       mx = fmaxf(mx, __shfl_xor(mx, 32));
-      const float base = (mx == -INFINITY ? 0.f : mx) - kBias;
+      const float base = mx == -INFINITY ? 0.f : mx;
       if (__any(mx > m)) {
-        const float a = exp2f(m - (base + kBias));
+        const float a = exp2f(m - base);
         l *= a;
   #pragma unroll
         for (int k = 0; k < S::U * S::VE; ++k) o[k] *= a;
@@ -227,7 +227,7 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
       for (int t = 0; t < S::NS; ++t)
   #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[t][e] = exp2f(x[t][e] - base);
+          x[t][e] = exp2f(x[t][e] - base + kBias);
           l += x[t][e];
         }
       Frag pf;
@@ -333,8 +333,8 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
       const int rk = row_a + k;
       const int64_t tk = chunk.t0 + rk / G;
       const int hk = kh * G + rk % G;
-      row_anew<DT, HD, S::T>(
-          C, A, s, kh, tk, hk, chunk.p0 + rk / G, range, lo, hi, base - kBias,
+      row_anew<DT, HD, S::T, true>(
+          C, A, s, kh, tk, hk, chunk.p0 + rk / G, range, lo, hi, top, kBias,
           sum == 0.f ? 0.f : 1.f / sum,
           whole ? nullptr : A.part_o + ((tk * A.heads + hk) * A.n_split + blockIdx.x) * HD,
           [](int) { return true; });

@@ -244,6 +244,56 @@ def test_attention_extreme_scores(dt, gpu_device):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("bits", [19, 20, 24, 25, 26, 27, 28, 31, 40, 100])
+def test_attention_scores_of_any_size(dt, hd, sign, bits, gpu_device):
+    """Scores of a single exact product, about 2^bits and 2^(bits - 7) apart: a row is
+    the mean of the values at its largest ones. Few rows, many, one token each, and
+    rows taken anew beside an infinity that only the last token sees."""
+    import ssalaad_amd as sa
+
+    dev, dtype, g = gpu_device, DT[dt], torch.Generator().manual_seed(bits)
+    tokens = 560 if dt == "f32" else 100  # of 8 heads: many rows
+    lens = [tokens + 70]
+    table, pages = pc.pages_of(lens, 16, g)
+    kp, vp = pc.cache(pages, 1, 16, hd, dtype, g)
+    level = 1024 + 8 * torch.randint(0, 8, (pages, 1, 16), generator=g)
+    kp[..., 0] = level.to(dtype)
+    q = torch.zeros(tokens, 8, hd, dtype=dtype)
+    q[..., 0] = sign * 1024
+    at = torch.arange(lens[0])
+    page = table[0].long()[at // 16]
+    x = (sign * level[page, 0, at % 16]).double()
+    v = vp[page, 0, at % 16].double()
+    want, size = torch.empty(tokens, hd).double(), torch.empty(tokens, hd).double()
+    for t in range(tokens):
+        top = x[: 71 + t] == x[: 71 + t].max()
+        want[t], size[t] = v[: 71 + t][top].mean(0), v[: 71 + t][top].abs().mean(0)
+    # the weights' rounding (equal, if not all to 1), fp32 sums, the output's rounding
+    tol = (2 * pc.u(dtype) + pc.F32 * (lens[0] + 64)) * size + pc.u(dtype) * want.abs()
+    tol = 1.01 * tol + (lens[0] * 2.0 ** -25 * v.abs().amax(0) if dt == "f16" else 0) + 1e-30
+    L = torch.tensor(lens, dtype=torch.int32, device=dev)
+    kd, vd, td = kp.to(dev), vp.to(dev), table.to(dev)
+    kw = dict(scale=2.0 ** (bits - 20))
+
+    def close(out, rows, what):
+        _close(out.cpu().double().amin(1), want[rows], tol[rows], what)
+        _close(out.cpu().double().amax(1), want[rows], tol[rows], what)
+
+    for n in (tokens, 3):
+        cu = torch.tensor([0, n], dtype=torch.int32, device=dev)
+        out = sa.paged_prompt_attention(q[-n:].to(dev), kd, vd, td, L, cu, **kw)
+        close(out, slice(tokens - n, tokens), (n, "prompt"))
+        vd[table[0, -1].item(), 0, (lens[0] - 1) % 16, 5] = float("inf")
+        out = sa.paged_prompt_attention(q[-n:].to(dev), kd, vd, td, L, cu, **kw)
+        close(out[:-1], slice(tokens - n, tokens - 1), (n, "prompt beside an infinity"))
+        vd.copy_(vp)
+    close(sa.paged_decode_attention(q[-1:].to(dev), kd, vd, td, L, **kw),
+          slice(tokens - 1, tokens), "decode")
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("scale", [0.0, 1e-44, 1e-46, -1e-46, 5e-324])
 def test_attention_of_a_vanishing_scale(dt, scale, gpu_device):
     """Means of what is seen, in every kernel: few rows, many, one token each."""
