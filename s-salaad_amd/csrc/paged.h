@@ -124,6 +124,12 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
   }
 }
 
+// The 16-bit element in the low half of x.
+template <int DT>
+__device__ __forceinline__ float low16(uint32_t x) {
+  return DT == DT_BF16 ? bf16_to_f32(x & 0xffffu) : f16_to_f32(x & 0xffffu);
+}
+
 // A product rounded before it is used (and not fused into what uses it).
 __device__ __forceinline__ float rounded(float x) {
   asm("" : "+v"(x));

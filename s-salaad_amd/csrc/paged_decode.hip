@@ -13,6 +13,12 @@
 //               operand passes through LDS. A lane reads 16-byte pieces of the
 //               8 (fp32: 4) keys it contracts and transposes them in registers.
 //
+// 16-bit products take a weight as two numbers of the type, itself rounded and what
+// that left. Memory bounds the kernel, so the second product costs little (nothing of
+// 91 µs at 60001 positions, 1 of 98 with a window of 1024, 0.3 of 15.4 at 16 sequences
+// of 1000), and outputs are as far from 64 bits as one rounding of the result makes
+// them; with one number 5 to 9% farther.
+//
 // A wave takes every NW-th tile of its workgroup's part of the context and
 // keeps its own running maximum, sum and output; the waves are joined through
 // LDS, the parts of a split context by join_kernel: a second launch, 4 to 5 µs,
@@ -230,15 +236,16 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
           x[t][e] = exp2f(x[t][e] - base + kBias);
           l += x[t][e];
         }
-      Frag pf;
+      Frag pf, pl;  // the weights; what their rounding left
       if constexpr (DT == DT_F32) {
   #pragma unroll
         for (int e = 0; e < 4; ++e) pf.f[e] = x[0][e];
       } else {
   #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          pf.d[2 * t] = pack2<DT>(x[t][0], x[t][1]);
-          pf.d[2 * t + 1] = pack2<DT>(x[t][2], x[t][3]);
+        for (int i = 0; i < 4; ++i) {
+          const float a = x[i / 2][2 * (i % 2)], b = x[i / 2][2 * (i % 2) + 1];
+          pf.d[i] = pack2<DT>(a, b);
+          pl.d[i] = pack2<DT>(a - low16<DT>(pf.d[i]), b - low16<DT>(pf.d[i] >> 16));
         }
       }
   #pragma unroll
@@ -258,6 +265,7 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
             }
           }
           M::run(o[w * S::VE + f], vf, pf);
+          if constexpr (DT != DT_F32) M::run(o[w * S::VE + f], vf, pl);
         }
     }
 

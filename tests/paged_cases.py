@@ -77,6 +77,27 @@ def attention(q, k_pool, v_pool, table, owners, positions, page, window=0, sinks
     return out, tol
 
 
+def attention_parts(q, k_pool, v_pool, table, owners, positions, page):
+    """(out, size, spread, other) in float64: the softmax average of what each token
+    sees, Σ p |v|, Σ p |v − out|, and the bound of a kernel's error from its fp32
+    scores, exponentials and sums and the rounding of its result."""
+    dt, hd, heads, kv = q.dtype, q.shape[2], q.shape[1], k_pool.shape[1]
+    out, size, spread, other = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(4))
+    for t in range(q.shape[0]):
+        row, p = table[owners[t]].long(), int(positions[t])
+        at = torch.arange(p + 1)
+        k, v = (x[row[at // page], :, at % page].double().repeat_interleave(heads // kv, 1)
+                for x in (k_pool, v_pool))
+        x = (q[t].double() * k).sum(-1).t() * hd ** -0.5
+        w = torch.softmax(x, -1).t()[..., None]
+        out[t], size[t] = (w * v).sum(0), (w * v.abs()).sum(0)
+        spread[t] = (w * (v - out[t]).abs()).sum(0)
+        mag = (q[t].double().abs() * k.abs()).sum(-1).amax(0) * hd ** -0.5
+        score = 2 * F32 * ((hd + 8) * mag + x.abs().amax(-1))
+        other[t] = (score + F32 * (p + 65))[:, None] * size[t] * 1.01 + u(dt) * out[t].abs() * 1.01
+    return out, size, spread, other + torch.finfo(dt).tiny
+
+
 def rotated(x, norm, eps, cos, sin, pos):
     """(x', tol) of paged_append for x [tokens, heads, hd]."""
     dt, hd = x.dtype, x.shape[-1]

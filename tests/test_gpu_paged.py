@@ -80,6 +80,33 @@ def test_decode_long_ragged(dt, page, gpu_device):
     _attend(gpu_device, DT[dt], 8, 2, 128, page, [5003, 1, 1024, 4097], poison=True, seed=page)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("counts", [None, [2, 1, 3]])  # one token each; chunks of few rows
+def test_few_rows_lose_no_digits_of_their_weights(dt, hd, counts, gpu_device):
+    """Outputs as close as one rounding: a weight in two numbers of the type is off by
+    its u squared, or by half the least step of the 256-fold fp16 ones."""
+    import ssalaad_amd as sa
+
+    dev, dtype, g = gpu_device, DT[dt], torch.Generator().manual_seed(hd)
+    lens = [717, 40, 3]
+    table, pages = pc.pages_of(lens, 16, g)
+    kp, vp = pc.cache(pages, 2, 16, hd, dtype, g)
+    owners, pos = pc.chunk_rows(counts or [1, 1, 1], lens)
+    q = (2 * torch.randn(len(owners), 4, hd, generator=g)).to(dtype)
+    want, size, _, other = pc.attention_parts(q, kp, vp, table, owners, pos, 16)
+    d = [t.to(dev) for t in (q, kp, vp, table, torch.tensor(lens, dtype=torch.int32))]
+    if counts is None:
+        got = sa.paged_decode_attention(*d)
+    else:
+        cu = torch.tensor([0] + counts).cumsum(0).int().to(dev)
+        got = sa.paged_prompt_attention(*d, cu, max_tokens=3, max_length=717)
+    tol = 1.01 * pc.u(dtype) ** 2 * size + other
+    if dt == "f16":
+        tol = tol + 717 * 2.0 ** -33 * vp.double().abs().max()
+    _close(got, want, tol)
+
+
 @pytest.mark.parametrize("bound", [1, 100, None])
 def test_decode_bound_shapes_only_the_launch(bound, gpu_device):
     _attend(gpu_device, torch.bfloat16, 8, 8, 64, 16, [2000, 3], max_length=bound)
