@@ -341,9 +341,8 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
       const int rk = row_a + k;
       const int64_t tk = chunk.t0 + rk / G;
       const int hk = kh * G + rk % G;
-      row_anew<DT, HD, S::T, true>(
-          C, A, s, kh, tk, hk, chunk.p0 + rk / G, range, lo, hi, top, kBias,
-          sum == 0.f ? 0.f : 1.f / sum,
+      row_anew<DT, HD, S::T>(
+          C, A, s, kh, tk, hk, chunk.p0 + rk / G, range, lo, hi, sum,
           whole ? nullptr : A.part_o + ((tk * A.heads + hk) * A.n_split + blockIdx.x) * HD,
           [](int) { return true; });
     }

@@ -37,26 +37,22 @@ __device__ __forceinline__ int row_parts(const PagedCache& C, const AttnArgs& A,
 // The tiles' products give a masked position the weight 0, which takes a NaN or an
 // infinity among its values into the row all the same. A row whose output is not
 // finite is therefore taken anew over tiles lo … hi − 1, by a wave, from the
-// positions that it sees alone, with the maximum `m` and sum that it has (the
-// scores of masked positions never entered those) and its kernel's formula for the
-// weights: 2^bias-fold, of scores rounded first (ROUND) or only far from zero. (600 tokens of 2 heads of 128, all
+// positions that it sees alone: their average, which a part holds times its sum `l`
+// (scores of masked positions never entered that). (600 tokens of 2 heads of 128, all
 // values NaN: 640 µs, finite 21; 4096 tokens of 16 heads 22 ms, 90 µs.)
 // part: where the row's part goes, or null for the output; mine(f): the features to
 // write.
-template <int DT, int HD, int T, bool ROUND, typename F>
+template <int DT, int HD, int T, typename F>
 __device__ __forceinline__ void row_anew(const PagedCache& C, const AttnArgs& A, int s, int kh,
                                          int64_t token, int head, int p, const TileRange& range,
-                                         int lo, int hi, float m, float bias, float inv,
-                                         float* part, F mine) {
+                                         int lo, int hi, float l, float* part, F mine) {
   constexpr int N = HD / 64, EB = Elem<DT>::bytes;
   const int lane = threadIdx.x & 63, f0 = lane * N;
   const char* q = A.q + (token * A.q_token + (int64_t)head * A.q_head) * EB;
   const int32_t* row = C.table + (int64_t)s * C.table_stride;
   const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
   const float sign = A.flip ? -A.scale_log2 : A.scale_log2;
-  const float top = m == -INFINITY ? 0.f : m;
-  const bool round = ROUND || fabsf(top) >= kFarScore;
-  float o[N];
+  float o[N], m = -INFINITY, sum = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) o[i] = 0.f;
   for (int i = lo; i < hi; ++i) {
@@ -75,8 +71,16 @@ __device__ __forceinline__ void row_anew(const PagedCache& C, const AttnArgs& A,
       for (int e = 0; e < 16 / EB; ++e)
         x = fmaf(A.keep ? load_scalar<DT>(&a, e) : 0.f, load_scalar<DT>(&b, e), x);
     }
-    const float y = round ? rounded(x * sign) - top + bias : fmaf(x, sign, bias - top);
-    const float w = see ? exp2f(y) : 0.f;
+    x = see ? rounded(x * sign) : -INFINITY;
+    float top = fmaxf(m, x);
+#pragma unroll
+    for (int b = 1; b < 64; b <<= 1) top = fmaxf(top, __shfl_xor(top, b));
+    const float base = top == -INFINITY ? 0.f : top, a = exp2f(m - base);
+    const float w = exp2f(x - base);
+    m = top;
+    sum = fmaf(sum, a, w);
+#pragma unroll
+    for (int j = 0; j < N; ++j) o[j] *= a;
     // values: a lane N features; a position not seen reads page 0 and counts as zero
     const uint64_t seen = __ballot(see);
     if (!seen) continue;
@@ -93,13 +97,16 @@ __device__ __forceinline__ void row_anew(const PagedCache& C, const AttnArgs& A,
     }
   }
 #pragma unroll
+  for (int b = 1; b < 64; b <<= 1) sum += __shfl_xor(sum, b);
+  const float by = sum == 0.f ? 0.f : (part ? l : 1.f) / sum;
+#pragma unroll
   for (int i = 0; i < N; ++i) {
     const int f = f0 + i;
     if (!mine(f)) continue;
     const int64_t at = (token * A.heads + head) * HD + f;
-    if (part) part[f] = o[i];
-    else if constexpr (DT == DT_F32) ((float*)A.out)[at] = o[i] * inv;
-    else ((uint16_t*)A.out)[at] = (uint16_t)to_bits<DT>(o[i] * inv);
+    if (part) part[f] = o[i] * by;
+    else if constexpr (DT == DT_F32) ((float*)A.out)[at] = o[i] * by;
+    else ((uint16_t*)A.out)[at] = (uint16_t)to_bits<DT>(o[i] * by);
   }
 }
 

@@ -20,10 +20,16 @@
 // workgroup 3800 cycles, in which a SIMD's two waves hold the matrix unit for 2048
 // and the vector unit for about as long; leaving out the loads, the exponentials,
 // the sums or a product's three quarters saves 9 µs, 5, 3 or 13 each, so no one
-// unit is the bound. (The teams half a round apart, by a second barrier: 3 µs more.
-// Row sums by a two-element dot product of the rounded weights: 0.6 less, not kept.)
+// unit is the bound. (The teams half a round apart, by a second barrier: 3 µs more.)
 // Beside the rounds a workgroup takes 14000 cycles, 5000 of them for its first
 // tile and q to arrive.
+//
+// 16-bit products take the weights rounded to the type; a row's sum is of the same
+// rounded weights, two a dot product, so that their errors cancel where few weights
+// carry a row: 4096 tokens are 2.04e-3 (rms) from 64 bits, at most 2.4e-3 of the
+// largest, where one rounding of the result makes 1.65e-3 and 2.2e-3; with a sum of
+// unrounded weights 2.14e-3 and 4.0e-3 in the same time. (Weights in two numbers, as
+// few rows have them: 1.65e-3, and 117 µs for 93, launch after launch.)
 //
 // K and V go from memory into LDS directly, a tile ahead of its use, two
 // buffers a team, one barrier a tile. LDS rows are permuted in 16-byte chunks by
@@ -107,6 +113,18 @@ __device__ __forceinline__ uint2 read8(uint32_t lds) {
   return __builtin_bit_cast(uint2, *(__attribute__((address_space(3))) u32x2*)(uintptr_t)lds);
 }
 
+// to and the two 16-bit elements of a pair
+template <int DT>
+__device__ __forceinline__ float sum2(uint32_t pair, float to) {
+  if constexpr (DT == DT_BF16) {
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, pair),
+                                           bf16x2{(__bf16)1.f, (__bf16)1.f}, to, false);
+  } else {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, pair),
+                                  f16x2{(_Float16)1.f, (_Float16)1.f}, to, false);
+  }
+}
 template <int DT>
 __device__ __forceinline__ void mma(f32x16& acc, const uint4& a, const uint4& b) {
   if constexpr (DT == DT_BF16)
@@ -448,7 +466,7 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
       const float y = __builtin_amdgcn_exp2f(kRoundAll ? rounded(z * scale) - top + kBias
                                                        : fmaf(z, scale, -base));
       x[i >> 4][i & 15] = y;
-      l += y;
+      if constexpr (T::F32) l += y;
     };
     if constexpr (T::F32) {
 #pragma unroll
@@ -477,8 +495,13 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
       auto packed = [&](int j) {
         const f32x16& y = x[j >> 1];
         const int e = 8 * (j & 1);
-        return uint4{pack2<DT>(y[e], y[e + 1]), pack2<DT>(y[e + 2], y[e + 3]),
-                     pack2<DT>(y[e + 4], y[e + 5]), pack2<DT>(y[e + 6], y[e + 7])};
+        const uint4 r{pack2<DT>(y[e], y[e + 1]), pack2<DT>(y[e + 2], y[e + 3]),
+                      pack2<DT>(y[e + 4], y[e + 5]), pack2<DT>(y[e + 6], y[e + 7])};
+        l = sum2<DT>(r.x, l);
+        l = sum2<DT>(r.y, l);
+        l = sum2<DT>(r.z, l);
+        l = sum2<DT>(r.w, l);
+        return r;
       };
 #pragma unroll
       for (int i = 0; i < 8; ++i) weight(i);
@@ -668,10 +691,9 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
     const int c = __builtin_ctz(anew), rc = r_a + c;
     const int64_t tc = chunk.t0 + rc / G;
     const int hc = kh * G + rc % G;
-    const float mc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(m), c));
-    const float ic = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(inv), c));
-    row_anew<DT, HD, T::KT, kRoundAll>(
-        C, A, s, kh, tc, hc, chunk.p0 + rc / G, range, lo, hi, mc, kBias, ic,
+    const float lc = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(l), c));
+    row_anew<DT, HD, T::KT>(
+        C, A, s, kh, tc, hc, chunk.p0 + rc / G, range, lo, hi, lc,
         whole ? nullptr : A.part_o + ((tc * A.heads + hc) * A.n_split + split) * HD,
         [&](int f) {  // the team's own
           return T::TEAMS == 1 || (T::F32 ? f / HALF % 2 : f / (HD / 2)) == team;

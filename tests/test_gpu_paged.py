@@ -107,6 +107,34 @@ def test_few_rows_lose_no_digits_of_their_weights(dt, hd, counts, gpu_device):
     _close(got, want, tol)
 
 
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("infinity", [False, True])
+def test_a_rows_sum_is_of_its_rounded_weights(dt, hd, infinity, gpu_device):
+    """Many rows: a weight's rounding moves the result by its distance from its value,
+    not by the value, also in rows taken anew beside an infinity of the last token."""
+    import ssalaad_amd as sa
+
+    dev, dtype, g = gpu_device, DT[dt], torch.Generator().manual_seed(hd)
+    lens, counts = [230], [90]
+    table, pages = pc.pages_of(lens, 16, g)
+    kp, vp = pc.cache(pages, 1, 16, hd, dtype, g)
+    vp = vp + 8  # values far from zero beside their spread
+    q = (2 * torch.randn(90, 8, hd, generator=g)).to(dtype)
+    owners, pos = pc.chunk_rows(counts, lens)
+    want, _, spread, other = pc.attention_parts(q, kp, vp, table, owners, pos, 16)
+    vd = vp.clone()
+    if infinity:
+        vd[table[0, 229 // 16], 0, 229 % 16, ::7] = float("inf")
+    d = [t.to(dev) for t in (q, kp, vd, table, torch.tensor(lens, dtype=torch.int32))]
+    got = sa.paged_prompt_attention(*d, torch.tensor([0, 90], dtype=torch.int32, device=dev))
+    tol = 1.01 * pc.u(dtype) * spread + other
+    if dt == "f16":  # 16-fold weights below half their least step
+        tol = tol + 2 * 230 * 2.0 ** -29 * vp.double().abs().max()
+    n = 89 if infinity else 90
+    _close(got[:n], want[:n], tol[:n])
+
+
 @pytest.mark.parametrize("bound", [1, 100, None])
 def test_decode_bound_shapes_only_the_launch(bound, gpu_device):
     _attend(gpu_device, torch.bfloat16, 8, 8, 64, 16, [2000, 3], max_length=bound)
