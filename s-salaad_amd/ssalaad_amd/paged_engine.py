@@ -5,7 +5,7 @@ sequence. `PagedEngine` runs prompts as a whole, keeps every sequence's keys and
 values in pages of one pool, lets sequences fork (sharing their common pages),
 end and be packed together, and scores tokens:
 
-  per layer   add_rmsnorm -> q,k,v in one fused SLR launch -> paged_append ->
+  per layer   add_rmsnorm (the embedding gather at layer 0) -> q,k,v in one fused SLR launch -> paged_append ->
               paged_prompt_attention / paged_decode_attention -> o_proj ->
               add_rmsnorm -> gate,up -> silu·up -> down_proj
   then        the final add_rmsnorm, the LM head (a plain library GEMM) and,
@@ -148,6 +148,23 @@ class PagedEngine:
         return live
 
     # ------------------------------------------------------------------ model
+    def _tokens(self, tokens) -> torch.Tensor:
+        """Token ids, 1-D int64 on the device; those given on the host are checked."""
+        t = torch.as_tensor(tokens, dtype=torch.int64).reshape(-1)
+        if not t.is_cuda and t.numel() and (int(t.min()) < 0 or int(t.max()) >= self.embed.shape[0]):
+            raise ValueError(f"token ids must lie in [0, {self.embed.shape[0]})")
+        return t.to(self.device)
+
+    def _embed_rmsnorm(self, tokens, w):
+        h = torch.empty(tokens.numel(), self.embed.shape[1], dtype=self.dtype, device=self.device)
+        out = torch.empty_like(h)
+        rc = self.lib.ssl_embed_rmsnorm(
+            self.embed.data_ptr(), self.embed.stride(0), self.embed.shape[0], tokens.data_ptr(),
+            h.data_ptr(), h.stride(0), w.data_ptr(), out.data_ptr(), out.stride(0), h.shape[0],
+            h.shape[1], self.eps, _lib.dtype_code(self.dtype), _lib.stream_ptr(self.device))
+        _lib.check(rc, "ssl_embed_rmsnorm")
+        return h, out
+
     def _add_rmsnorm(self, h, delta, w):
         out = torch.empty_like(h)
         rc = self.lib.ssl_add_rmsnorm(
@@ -185,10 +202,11 @@ class PagedEngine:
                 ends.append(ends[-1] + n)
             cu = self._ints(ends)
         n, H, KH, hd = tokens.numel(), self.heads, self.kv_heads, self.head_dim
-        h = self.embed[tokens]
-        delta = None
         for i, L in enumerate(self.layers):
-            x = self._add_rmsnorm(h, delta, L.in_norm)
+            if i == 0:
+                h, x = self._embed_rmsnorm(tokens, L.in_norm)
+            else:
+                x = self._add_rmsnorm(h, delta, L.in_norm)
             q, k, v = L.qkv(x)
             q = paged_append(q.view(n, H, hd), k.view(n, KH, hd), v.view(n, KH, hd), self.cos,
                              self.sin, self.k_pool[i], self.v_pool[i], self.table, owners,
@@ -208,9 +226,10 @@ class PagedEngine:
     def feed(self, seqs, tokens, *, all_logits: bool = False):
         """Append tokens to sequences: tokens[i], a 1-D int64 tensor or a list, to
         seqs[i]. Returns the logits after each sequence's last token [n, vocab],
-        or with all_logits those after every token [tokens, vocab]."""
+        or with all_logits those after every token [tokens, vocab]. Ids on the host
+        are checked; one on the device that no embedding has counts as a zero row."""
         seqs = self._names(seqs)
-        parts = [torch.as_tensor(t, dtype=torch.int64).reshape(-1).to(self.device) for t in tokens]
+        parts = [self._tokens(t) for t in tokens]
         counts = [t.numel() for t in parts]
         if len(parts) != len(seqs) or min(counts, default=0) < 1:
             raise ValueError("every sequence takes one or more tokens")
@@ -226,13 +245,13 @@ class PagedEngine:
         seqs = self._names(seqs)
         if tokens.shape != (len(seqs),):
             raise ValueError(f"a step takes {len(seqs)} tokens, one a sequence")
-        return self.lm_head(self._forward(tokens.to(self.device), seqs, [1] * len(seqs)))
+        return self.lm_head(self._forward(self._tokens(tokens), seqs, [1] * len(seqs)))
 
     @torch.no_grad()
     def score(self, seq: int, tokens, *, top: int = 0) -> TokenLogprobs:
         """Feed `tokens` to an ended sequence and score each after the first under
         the ones before it."""
-        tokens = torch.as_tensor(tokens, dtype=torch.int64).reshape(-1).to(self.device)
+        tokens = self._tokens(tokens)
         if self._host_lengths[self._names([seq])[0]]:
             raise ValueError("scores are of a sequence's first tokens; free it before")
         logits = self.feed([seq], [tokens], all_logits=True)

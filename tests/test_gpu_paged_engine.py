@@ -147,3 +147,36 @@ def test_the_example_serves_candidates(gpu_device):
         for t in tokens[:1]])
     # 20 fp32 log probabilities of logits within the tolerance of each other
     assert torch.allclose(again, logprobs[:1], atol=20 * 1e-4)
+
+
+def test_tokens_without_an_embedding(gpu_device):
+    """Refused where the host can see them, a zero row where only the device can; never
+    an index past the embeddings."""
+    from ssalaad_amd import PagedEngine
+
+    eng = PagedEngine(_model("llama").to(gpu_device), max_seqs=2, pages=8, page=16)
+    for bad in ([5, 300], [-1], torch.tensor([2 ** 40])):
+        with pytest.raises(ValueError, match="token ids"):
+            eng.feed([0], [bad])
+        with pytest.raises(ValueError, match="token ids"):
+            eng.score(0, bad)
+    with pytest.raises(ValueError, match="token ids"):
+        eng.step([0], torch.tensor([300]))
+    assert int(eng.lengths.abs().sum()) == 0 and int(eng.refs.abs().sum()) == 0
+    ids = torch.tensor([7, 300, -5, 2 ** 40], device=gpu_device)
+    got = eng.feed([0], [ids], all_logits=True)
+    assert bool(got.isfinite().all())
+    alone = eng.feed([1], [[7]])
+    assert _err(got[:1], alone.double().cpu()) <= TOL
+    # the first row is the embedding's, the others are zeros
+    h, x = eng._embed_rmsnorm(ids, eng.layers[0].in_norm)
+    assert torch.equal(h[0], eng.embed[7]) and not h[1:].any() and not x[1:].any()
+
+
+def test_int32_tokens_step(gpu_device):
+    from ssalaad_amd import PagedEngine
+
+    eng = PagedEngine(_model("llama").to(gpu_device), max_seqs=2, pages=8, page=16)
+    a = eng.step([0], torch.tensor([9], dtype=torch.int32))
+    b = eng.step([1], torch.tensor([9], device=gpu_device))
+    assert torch.equal(a, b)
