@@ -82,7 +82,10 @@ class PagedEngine:
         self.table = torch.full((max_seqs, cols), -1, dtype=torch.int32, device=dev)
         self.lengths = torch.zeros(max_seqs, dtype=torch.int32, device=dev)
         self.refs = torch.zeros(pages, dtype=torch.int32, device=dev)
+        # each sequence's length and pages; a call that fails leaves the lengths, and
+        # the pages it reserved to the sequence
         self._host_lengths = [0] * max_seqs
+        self._host_pages = [0] * max_seqs
         with torch.no_grad():
             pos = torch.arange(self.max_context, device=dev)[None]
             cos, sin = rot(torch.zeros(1, dtype=torch.float32, device=dev), position_ids=pos)
@@ -105,11 +108,10 @@ class PagedEngine:
         """Pages for `counts` more positions of each sequence."""
         rows, cols = [], []
         for s, n in zip(seqs, counts):
-            have = -(-self._host_lengths[s] // self.page)
             last = self._host_lengths[s] + n
             if last > self.max_context:
                 raise ValueError(f"sequence {s} would pass {self.max_context} positions")
-            new = range(have, -(-last // self.page))
+            new = range(self._host_pages[s], -(-last // self.page))
             rows += [s] * len(new)
             cols += new
         if not rows:
@@ -120,12 +122,17 @@ class PagedEngine:
         at = (torch.tensor(rows, device=self.device), torch.tensor(cols, device=self.device))
         self.table[at] = free.int()
         self.refs[free] = 1
+        for s in rows:
+            self._host_pages[s] += 1
 
     def fork(self, src, dst) -> None:
         """Let the ended sequences dst go on as src do."""
         src, dst = [int(s) for s in src], self._names(dst)
         if any(self._host_lengths[d] for d in dst):
             raise ValueError("a sequence can be forked into one that has ended only")
+        held = [d for d in dst if self._host_pages[d]]  # by a call that failed
+        if held:
+            self.free(held)
         out = fork_pages(self.table, self.lengths, self.refs, self.k_pool, self.v_pool,
                          self._ints(src), self._ints(dst))
         if not bool(out[3].all()):
@@ -133,6 +140,7 @@ class PagedEngine:
         self.table, self.lengths, self.refs = out[:3]
         for s, d in zip(src, dst):
             self._host_lengths[d] = self._host_lengths[s]
+            self._host_pages[d] = -(-self._host_lengths[s] // self.page)
 
     def free(self, seqs) -> None:
         """End sequences."""
@@ -140,7 +148,7 @@ class PagedEngine:
         self.table, self.lengths, self.refs = free_pages(self.table, self.lengths, self.refs,
                                                          self._ints(seqs))
         for s in seqs:
-            self._host_lengths[s] = 0
+            self._host_lengths[s] = self._host_pages[s] = 0
 
     def compact(self) -> torch.Tensor:
         """Move the pages in use to the lowest numbers; their count (0-d int32)."""
@@ -182,25 +190,34 @@ class PagedEngine:
         _lib.check(rc, "ssl_silu_mul")
         return out
 
+    def _logits(self, tokens: torch.Tensor, seqs: list[int], counts: list[int],
+                rows: torch.Tensor | None = None) -> torch.Tensor:
+        """Append new tokens, counts[i] of seqs[i]: their logits, or those of `rows`
+        of them. The sequences grow when all has been issued."""
+        x = self._forward(tokens, seqs, counts)
+        logits = self.lm_head(x if rows is None else x[rows])
+        ends = [self._host_lengths[s] + n for s, n in zip(seqs, counts)]
+        self.lengths[self._ints(seqs).long()] = self._ints(ends)
+        for s, n in zip(seqs, ends):
+            self._host_lengths[s] = n
+        return logits
+
     def _forward(self, tokens: torch.Tensor, seqs: list[int], counts: list[int]) -> torch.Tensor:
         """The final hidden states of new tokens, counts[i] of seqs[i]."""
         starts = [self._host_lengths[s] for s in seqs]
+        ends = [a + n for a, n in zip(starts, counts)]
         self._reserve(seqs, counts)
-        for s, n in zip(seqs, counts):
-            self._host_lengths[s] += n
         owners = self._ints([s for s, n in zip(seqs, counts) for _ in range(n)])
         positions = self._ints([a + j for a, n in zip(starts, counts) for j in range(n)])
-        rows = self._ints(seqs).long()
-        lengths = self._ints([self._host_lengths[s] for s in seqs])
-        self.lengths[rows] = lengths
-        table = self.table[rows]
-        longest = max(self._host_lengths[s] for s in seqs)
+        lengths = self._ints(ends)
+        table = self.table[self._ints(seqs).long()]
+        longest = max(ends)
         cu = None
         if max(counts) > 1:
-            ends = [0]
+            at = [0]
             for n in counts:
-                ends.append(ends[-1] + n)
-            cu = self._ints(ends)
+                at.append(at[-1] + n)
+            cu = self._ints(at)
         n, H, KH, hd = tokens.numel(), self.heads, self.kv_heads, self.head_dim
         for i, L in enumerate(self.layers):
             if i == 0:
@@ -233,11 +250,8 @@ class PagedEngine:
         counts = [t.numel() for t in parts]
         if len(parts) != len(seqs) or min(counts, default=0) < 1:
             raise ValueError("every sequence takes one or more tokens")
-        x = self._forward(torch.cat(parts), seqs, counts)
-        if not all_logits:
-            ends = torch.tensor(counts, device=self.device).cumsum(0) - 1
-            x = x[ends]
-        return self.lm_head(x)
+        last = None if all_logits else torch.tensor(counts, device=self.device).cumsum(0) - 1
+        return self._logits(torch.cat(parts), seqs, counts, last)
 
     @torch.no_grad()
     def step(self, seqs, tokens: torch.Tensor) -> torch.Tensor:
@@ -245,7 +259,7 @@ class PagedEngine:
         seqs = self._names(seqs)
         if tokens.shape != (len(seqs),):
             raise ValueError(f"a step takes {len(seqs)} tokens, one a sequence")
-        return self.lm_head(self._forward(self._tokens(tokens), seqs, [1] * len(seqs)))
+        return self._logits(self._tokens(tokens), seqs, [1] * len(seqs))
 
     @torch.no_grad()
     def score(self, seq: int, tokens, *, top: int = 0) -> TokenLogprobs:

@@ -180,3 +180,47 @@ def test_int32_tokens_step(gpu_device):
     a = eng.step([0], torch.tensor([9], dtype=torch.int32))
     b = eng.step([1], torch.tensor([9], device=gpu_device))
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("where", ["the lm head", "a layer"])
+def test_a_call_that_fails_changes_no_sequence(where, gpu_device):
+    """Nothing grows, no page is lost, and the call can be made again."""
+    from ssalaad_amd import PagedEngine
+
+    m = _model("llama").to(gpu_device)
+    eng = PagedEngine(m, max_seqs=4, pages=12, page=16)
+    ref = PagedEngine(m, max_seqs=4, pages=12, page=16)
+
+    def fail(*a):
+        raise torch.OutOfMemoryError("no memory")
+
+    def failing(call):
+        head, down = eng.lm_head, eng.layers[1].down
+        if where == "a layer":
+            eng.layers[1].down = fail
+        else:
+            eng.lm_head = fail
+        with pytest.raises(torch.OutOfMemoryError):
+            call()
+        eng.lm_head, eng.layers[1].down = head, down
+
+    text = list(range(40))
+    failing(lambda: eng.feed([0, 2], [text, text[:17]]))
+    assert int(eng.lengths.sum()) == 0
+    assert torch.equal(eng.feed([0, 2], [text, text[:17]]), ref.feed([0, 2], [text, text[:17]]))
+    assert int(eng.refs.sum()) == 5
+    for t in range(12):  # across a page's end
+        tok = torch.tensor([t, t + 1])
+        failing(lambda: eng.step([0, 2], tok))
+        assert torch.equal(eng.step([0, 2], tok), ref.step([0, 2], tok))
+    assert torch.equal(eng.lengths, ref.lengths) and int(eng.refs.sum()) == int(ref.refs.sum())
+    # a fork into a sequence that a failed call reserved pages for
+    failing(lambda: eng.feed([1], [text]))
+    eng.fork([0], [1])
+    ref.fork([0], [1])
+    tok = torch.tensor([3])
+    assert torch.equal(eng.step([1], tok), ref.step([1], tok))
+    assert int(eng.refs.sum()) == int(ref.refs.sum())
+    failing(lambda: eng.feed([3], [text[:20]]))
+    eng.free([0, 1, 2, 3])
+    assert int(eng.refs.abs().sum()) == 0 and int((eng.table != -1).sum()) == 0
