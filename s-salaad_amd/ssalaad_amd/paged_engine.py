@@ -128,6 +128,10 @@ class PagedEngine:
     def fork(self, src, dst) -> None:
         """Let the ended sequences dst go on as src do."""
         src, dst = [int(s) for s in src], self._names(dst)
+        if len(src) != len(dst):
+            raise ValueError(f"{len(src)} sequences to fork into {len(dst)}")
+        if not all(0 <= s < len(self._host_lengths) for s in src):
+            raise ValueError(f"sequences must lie in [0, {len(self._host_lengths)})")
         if any(self._host_lengths[d] for d in dst):
             raise ValueError("a sequence can be forked into one that has ended only")
         held = [d for d in dst if self._host_pages[d]]  # by a call that failed

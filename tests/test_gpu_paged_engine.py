@@ -224,3 +224,16 @@ def test_a_call_that_fails_changes_no_sequence(where, gpu_device):
     failing(lambda: eng.feed([3], [text[:20]]))
     eng.free([0, 1, 2, 3])
     assert int(eng.refs.abs().sum()) == 0 and int((eng.table != -1).sum()) == 0
+
+
+def test_forks_of_no_such_sequence_are_refused(gpu_device):
+    from ssalaad_amd import PagedEngine
+
+    eng = PagedEngine(_model("llama").to(gpu_device), max_seqs=3, pages=8, page=16)
+    eng.feed([2], [[1, 2, 3]])
+    for src, dst in (([-1], [0]), ([3], [0]), ([2], [0, 1]), ([2, 2], [0])):
+        with pytest.raises(ValueError):
+            eng.fork(src, dst)
+    assert eng.lengths.tolist() == [0, 0, 3] and int(eng.refs.sum()) == 1
+    eng.fork([2, 2], [0, 1])
+    assert eng.lengths.tolist() == [3, 3, 3] and int(eng.refs.sum()) == 3
