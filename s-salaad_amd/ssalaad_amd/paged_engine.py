@@ -19,6 +19,8 @@ waits for the device (for the free pages' numbers).
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch import nn
 
@@ -27,6 +29,15 @@ from .decode import _group, _Layer
 from .logprobs import TokenLogprobs, token_logprobs
 from .paged import (compact_pages, fork_pages, free_pages, paged_append, paged_decode_attention,
                     paged_prompt_attention)
+
+
+def _on_device(method):
+    """The method with the engine's device as torch's current one, without gradients."""
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        with torch.cuda.device(self.device), torch.no_grad():
+            return method(self, *args, **kw)
+    return call
 
 
 class PagedEngine:
@@ -125,6 +136,7 @@ class PagedEngine:
         for s in rows:
             self._host_pages[s] += 1
 
+    @_on_device
     def fork(self, src, dst) -> None:
         """Let the ended sequences dst go on as src do."""
         src, dst = [int(s) for s in src], self._names(dst)
@@ -146,6 +158,7 @@ class PagedEngine:
             self._host_lengths[d] = self._host_lengths[s]
             self._host_pages[d] = -(-self._host_lengths[s] // self.page)
 
+    @_on_device
     def free(self, seqs) -> None:
         """End sequences."""
         seqs = self._names(seqs)
@@ -154,6 +167,7 @@ class PagedEngine:
         for s in seqs:
             self._host_lengths[s] = self._host_pages[s] = 0
 
+    @_on_device
     def compact(self) -> torch.Tensor:
         """Move the pages in use to the lowest numbers; their count (0-d int32)."""
         self.table, self.refs, live = compact_pages(self.table, self.refs, self.k_pool, self.v_pool)
@@ -243,7 +257,7 @@ class PagedEngine:
             delta = L.down(self._silu_mul(*L.gu(x)))
         return self._add_rmsnorm(h, delta, self.norm)
 
-    @torch.no_grad()
+    @_on_device
     def feed(self, seqs, tokens, *, all_logits: bool = False):
         """Append tokens to sequences: tokens[i], a 1-D int64 tensor or a list, to
         seqs[i]. Returns the logits after each sequence's last token [n, vocab],
@@ -257,7 +271,7 @@ class PagedEngine:
         last = None if all_logits else torch.tensor(counts, device=self.device).cumsum(0) - 1
         return self._logits(torch.cat(parts), seqs, counts, last)
 
-    @torch.no_grad()
+    @_on_device
     def step(self, seqs, tokens: torch.Tensor) -> torch.Tensor:
         """One token a sequence (tokens [n] int64): the logits [n, vocab]."""
         seqs = self._names(seqs)
@@ -265,7 +279,7 @@ class PagedEngine:
             raise ValueError(f"a step takes {len(seqs)} tokens, one a sequence")
         return self._logits(self._tokens(tokens), seqs, [1] * len(seqs))
 
-    @torch.no_grad()
+    @_on_device
     def score(self, seq: int, tokens, *, top: int = 0) -> TokenLogprobs:
         """Feed `tokens` to an ended sequence and score each after the first under
         the ones before it."""

@@ -237,3 +237,24 @@ def test_forks_of_no_such_sequence_are_refused(gpu_device):
     assert eng.lengths.tolist() == [0, 0, 3] and int(eng.refs.sum()) == 1
     eng.fork([2, 2], [0, 1])
     assert eng.lengths.tolist() == [3, 3, 3] and int(eng.refs.sum()) == 3
+
+
+def test_the_engine_runs_on_its_models_device(gpu_device, monkeypatch):
+    """Every call makes the model's device current for its launches."""
+    from ssalaad_amd import PagedEngine
+
+    entered = []
+
+    class Device(torch.cuda.device):
+        def __enter__(self):
+            entered.append(self.idx)
+            return super().__enter__()
+
+    eng = PagedEngine(_model("llama").to(gpu_device), max_seqs=3, pages=8, page=16)
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    for call in (lambda: eng.feed([0], [[1, 2]]), lambda: eng.step([0], torch.tensor([3])),
+                 lambda: eng.fork([0], [1]), lambda: eng.free([0]), lambda: eng.compact(),
+                 lambda: eng.score(2, [1, 2, 3])):
+        entered.clear()
+        call()
+        assert entered and set(entered) == {gpu_device.index}
