@@ -22,7 +22,7 @@ namespace {
 
 // Rows of one key/value head the kernel for few of them is considered for, which
 // reads a context once for 16. (500 tokens, 8 fp32 heads of 128: 20 µs, the other
-// 34; 8 chunks of 40 over 8000 positions, 16 heads of 64: 54 µs, the other 50. In
+// 34; 8 chunks of 40 over 8000 positions, 16 heads of 64: 55 µs, the other 48. In
 // 16 bits more rows are never its case: 300 tokens of a group of 4 over 2000
 // positions 26 µs, the other 20.)
 constexpr int few_rows(int dtype) { return dtype == SSL_F32 ? 4096 : 512; }

@@ -739,20 +739,24 @@ int launch_dt(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
 
 }  // namespace
 
-// Splits contexts where that is faster by an estimate of the launch: a round
-// (a tile a team) takes kRound µs with its share of what a workgroup does beside
-// them, the rows' workgroups run a device full at a time, and a join costs 4 µs and its parts' traffic at 3 TB/s. (2 prompts of
-// 1000 tokens, 16 heads of 128: whole 23 µs, in 2 parts 38; 500 tokens, 8 fp32
-// heads of 128: whole 74 µs, in 4 parts 35, in 8 32.) Fills n_split and per;
-// returns the parts' bytes.
+// Splits contexts where that is faster by an estimate of the launch: a round (a tile
+// a team) takes kRound µs with its share of what a workgroup does beside them, a
+// compute unit takes one workgroup at a time (64-wide heads leave LDS for two, but
+// their registers, 138 and 159, hold no more than 12 waves), and a join costs 4 µs and
+// its parts' traffic at 3 TB/s. A device full of 64-wide heads waits a third of its
+// last parts besides. (2 prompts of 1000 tokens, 16 heads of 128: whole 23 µs, in 2
+// parts 38; 500 tokens, 8 fp32 heads of 128: whole 74 µs, in 4 parts 35, in 8 32; 4096
+// tokens, 16 heads of 64: whole 64 µs, in 2 parts 112; 250 over 4000 positions, 16
+// heads of 64 over 4: whole 46 µs, in 6 parts 21.) Fills n_split and per; returns the
+// parts' bytes.
 int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t max_tokens,
                           int64_t max_length) {
   // by head_dim 64, 128, 256
-  static constexpr double kRound[2][3] = {{1.7, 2.2, 2.8}, {3.9, 7.6, 8.9}};
+  static constexpr double kRound[2][3] = {{1.4, 2.2, 2.8}, {5.5, 7.6, 8.9}};
   const bool f32 = dtype == SSL_F32;
   const int KT = f32 ? 32 : 64, G = A->heads / C.kv_heads;
   const int teams = C.head_dim == 256 ? 1 : 2;
-  const double slots = (double)device_cus() * (C.head_dim == 64 ? 2 : 1);
+  const double slots = (double)device_cus(), tail = C.head_dim == 64 ? 1. / 3 : 0.;
   const double round = kRound[f32][C.head_dim == 64 ? 0 : C.head_dim == 128 ? 1 : 2];
   const int64_t per_seq = std::max<int64_t>(1, (max_tokens * G + 127) / 128);
   const int64_t tiles = std::min<int64_t>(C.seqs * per_seq, A->tokens * G / 128 + C.seqs);
@@ -771,7 +775,7 @@ int64_t paged_prompt_plan(const PagedCache& C, AttnArgs* A, int dtype, int64_t m
     const int64_t per = (keys + n - 1) / n, parts = (keys + per - 1) / per;
     const double rounds = (double)((per + teams - 1) / teams);
     const double full = blocks * mean * keys / teams / slots;
-    const double us = round * std::max(rounds, full) + (parts > 1 ? 4 + parts * part_us : 0);
+    const double us = round * std::max(rounds, full + tail * rounds) + (parts > 1 ? 4 + parts * part_us : 0);
     if (n == 1 || us < best) {
       best = us;
       A->per = (int)std::min<int64_t>(per, 0x3fffffff);

@@ -73,6 +73,16 @@ def test_cache_descriptions_are_checked_before_any_launch():
     assert _lib.load().ssl_paged_attention(None, None) == 1
 
 
+@pytest.mark.parametrize("dt,tokens", [(_lib.SSL_BF16, 2048), (_lib.SSL_BF16, 4096), (_lib.SSL_F16, 4096)])
+def test_whole_prompts_that_fill_the_device_are_not_split(dt, tokens):
+    """16 heads of 64, a workgroup and more a compute unit: no parts, no workspace."""
+    st = paged._ATTENTION
+    pools = [FAKE, FAKE, 0, 16 * 16 * 64, 16 * 64, 64, 1, 300, 16, 16, 64]
+    args = st.pack(st.size, *pools, FAKE, 300, 1, 300, dt, FAKE, 1024, 64, FAKE, FAKE, FAKE, tokens, 16,
+                   0, 0, 0.125, tokens, tokens, 0, 0)
+    assert _lib.load().ssl_paged_attention_workspace_size(args) == 0
+
+
 def test_append_arguments_are_checked_before_any_launch():
     st = paged._APPEND
     base = [st.size, *POOLS, *GRID, _lib.SSL_BF16, FAKE, 256, 64, FAKE, 128, 64, FAKE, 128, 64,
