@@ -734,8 +734,9 @@ int ssl_paged_attention(const ssl_paged_attention_args* args, void* stream);
  *   ends once; one out of range is passed over.
  * ssl_pages_fork  dst[i] goes on as src[i] does: it shares the whole pages
  *   (their references grow) and, where the last page is partly filled, gets the
- *   lowest free page with those positions copied in every layer. Forks are
- *   served in order, all from the state before the call. ok[i] (one byte) is 0
+ *   lowest free page with those positions copied in every layer; pages that
+ *   dst's row still names lose that reference. Forks are served in order, all
+ *   from the state before the call. ok[i] (one byte) is 0
  *   and nothing changes where src or dst is out of range, dst is not empty
  *   (length 0) or named before, a page of src is out of range, or no page is
  *   free. `workspace`: ssl_pages_fork_workspace_size(n) bytes.

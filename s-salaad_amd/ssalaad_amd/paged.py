@@ -308,7 +308,7 @@ def fork_pages(table: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor,
     """Let sequence dst[i] (ended, length 0) go on as src[i] does:
     (table, lengths, refs, ok). Whole pages are shared; a partly filled last one
     is copied, in every layer, into the lowest free page (in place in the
-    pools). Forks are served in order, all from the state before the call. ok
+    pools); pages that dst's row still names lose that reference. Forks are served in order, all from the state before the call. ok
     [n] bool is False, and nothing changes, where src or dst is out of range,
     dst is not empty or was named before, a page of src is missing, or no page
     is free."""

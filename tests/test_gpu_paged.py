@@ -642,6 +642,25 @@ def test_fork_of_missing_pages_and_one_layer(gpu_device):
     assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
 
 
+def test_a_fork_gives_back_what_its_row_held(gpu_device):
+    """An empty sequence whose row names pages (reserved for it, say): the counts stay
+    those of the entries."""
+    import ssalaad_amd as sa
+
+    dev, g = gpu_device, torch.Generator().manual_seed(14)
+    table = torch.tensor([[3, 5, -1], [1, 9, 0], [2, -1, 3], [-1, -1, -1]], dtype=torch.int32)
+    lens = torch.tensor([20, 0, 0, 0], dtype=torch.int32)
+    refs = torch.tensor([1, 1, 1, 2, 0, 1, 0], dtype=torch.int32)
+    kp, vp = (t.to(dev) for t in pc.cache(7, 1, 16, 64, torch.bfloat16, g, layers=2))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    t, n, r, ok = sa.fork_pages(table.to(dev), lens.to(dev), refs.to(dev), kp, vp, i32(0, 0, 0),
+                                i32(1, 2, 1))
+    assert ok.tolist() == [True, True, False] and n.tolist() == [20, 20, 20, 0]
+    assert t.tolist() == [[3, 5, -1], [3, 4, -1], [3, 6, -1], [-1, -1, -1]]
+    held = t[t >= 0].long().cpu()
+    assert torch.equal(r.cpu().long(), torch.bincount(held, minlength=7))
+
+
 def test_many_forks_and_pages(gpu_device):
     """More forks and pages than one workgroup holds at a time, and more forks
     than free pages."""
