@@ -163,6 +163,20 @@ def test_prompt_window_and_sinks(dt, window, sinks, gpu_device):
 
 
 @pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n", [64, 65, 130, 200])
+def test_prompts_of_many_sequences(dt, n, gpu_device):
+    """More sequences than a wave has lanes, some without tokens; the rows of one of
+    them take the kernel for many rows."""
+    counts = pc.spread(9, n)
+    for i in (0, 5, 63, n - 2):
+        counts[i] = 0
+    counts[n // 2], counts[n - 1] = 140, 75
+    lens = [c + i % 7 if i % 3 else c for i, c in enumerate(counts)]
+    heads, kv = (8, 1) if dt != "f32" else (32, 1)
+    _attend(gpu_device, DT[dt], heads, kv, 64, 16, lens, counts=counts, poison=n == 65, seed=n)
+
+
+@pytest.mark.parametrize("dt", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("counts,lens", [([1], [3000]), ([5, 1], [2500, 1]), ([130], [1500]),
                                          ([300, 1, 2], [300, 900, 2])])
 def test_prompt_few_rows_over_long_contexts(dt, counts, lens, gpu_device):

@@ -258,3 +258,27 @@ def test_the_engine_runs_on_its_models_device(gpu_device, monkeypatch):
         entered.clear()
         call()
         assert entered and set(entered) == {gpu_device.index}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("model_type,hd", [("llama", 64), ("qwen3", 128)])
+def test_logits_in_16_bits(model_type, hd, dtype, gpu_device):
+    """A prompt, steps, a fork and a further chunk. Two layers round some ten times on
+    the way to the logits: within 16 roundings of the forward in float64 of the same
+    (rounded) weights, relative to the largest logit."""
+    from ssalaad_amd import PagedEngine
+
+    m = _model(model_type, hd).to(dtype)
+    ref = _model(model_type, hd).to(dtype).double()
+    eng = PagedEngine(m.to(gpu_device), max_seqs=3, pages=30, page=16)
+    g = torch.Generator().manual_seed(4)
+    text = torch.randint(0, 300, (90,), generator=g)
+    with torch.no_grad():
+        want = ref(text[None]).logits[0]
+    tol = 16 * torch.finfo(dtype).eps / 2
+    assert _err(eng.feed([0], [text[:61]], all_logits=True), want[:61]) <= tol
+    for t in range(61, 66):
+        assert _err(eng.step([0], text[t: t + 1]), want[t: t + 1]) <= tol
+    eng.fork([0], [2])
+    got = eng.feed([2, 0], [text[66:], text[66:70]], all_logits=True)
+    assert _err(got, torch.cat([want[66:], want[66:70]])) <= tol
