@@ -15,9 +15,9 @@
 //
 // 16-bit products take a weight as two numbers of the type, itself rounded and what
 // that left. Memory bounds the kernel, so the second product costs little (nothing of
-// 91 µs at 60001 positions, 1 of 98 with a window of 1024, 0.3 of 15.4 at 16 sequences
-// of 1000), and outputs are as far from 64 bits as one rounding of the result makes
-// them; with one number 5 to 9% farther.
+// 88 µs at 60001 positions, 2 of 94 with a window of 1024, nothing of 15.8 at 16
+// sequences of 1000), and outputs are as far from 64 bits as one rounding of the result
+// makes them; with one number 5 to 9% farther.
 //
 // A wave takes every NW-th tile of its workgroup's part of the context and
 // keeps its own running maximum, sum and output; the waves are joined through
@@ -27,7 +27,7 @@
 //
 // Measured: contexts of up to 60001 positions of 4 sequences, 32 heads over 8 of
 // 128, bf16: 88 µs, 4.86 TB/s (a large copy here: 4.83); 64 sequences, a window of
-// 1024, 16 heads: 94 µs, 4.76 TB/s. One sequence of 717, 16 heads of 64: 7.7 µs, the
+// 1024, 16 heads: 96 µs, 4.65 TB/s. One sequence of 717, 16 heads of 64: 7.8 µs, the
 // latency of a launch, of the table, of three loads in turn and of the join of waves.
 #include <hip/hip_runtime.h>
 #include <math.h>
@@ -233,7 +233,7 @@ void decode_kernel(PagedCache C, AttnArgs A, int n_blocks) {
       for (int t = 0; t < S::NS; ++t)
   #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          x[t][e] = exp2f(x[t][e] - base + kBias);
+          x[t][e] = __builtin_amdgcn_exp2f(kBias ? x[t][e] - base + kBias : x[t][e] - base);
           l += x[t][e];
         }
       Frag pf, pl;  // the weights; what their rounding left

@@ -39,7 +39,7 @@ __device__ __forceinline__ int row_parts(const PagedCache& C, const AttnArgs& A,
 // finite is therefore taken anew over tiles lo … hi − 1, by a wave, from the
 // positions that it sees alone: their average, which a part holds times its sum `l`
 // (scores of masked positions never entered that). (600 tokens of 2 heads of 128, all
-// values NaN: 640 µs, finite 21; 4096 tokens of 16 heads 22 ms, 90 µs.)
+// values NaN: 680 µs, finite 24; 4096 tokens of 16 heads 23 ms, 92 µs.)
 // part: where the row's part goes, or null for the output; mine(f): the features to
 // write.
 template <int DT, int HD, int T, typename F>

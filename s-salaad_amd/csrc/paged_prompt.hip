@@ -15,14 +15,16 @@
 //                in any order both operands share); V is transposed on its way
 //                out of LDS (ds_read_tr16), fp32 values are read as they are.
 //
-// What bounds it: 4096 tokens of one sequence, 16 heads of 128, bf16, take 80 µs,
-// 850 TFLOP/s (a large library product: 1157). A round of two tiles takes a
-// workgroup 3800 cycles, in which a SIMD's two waves hold the matrix unit for 2048
-// and the vector unit for about as long; leaving out the loads, the exponentials,
-// the sums or a product's three quarters saves 9 µs, 5, 3 or 13 each, so no one
-// unit is the bound. (The teams half a round apart, by a second barrier: 3 µs more.)
-// Beside the rounds a workgroup takes 14000 cycles, 5000 of them for its first
-// tile and q to arrive.
+// What bounds it: 4096 tokens of one sequence, 16 heads of 128, bf16, hold a compute
+// unit for 162000 cycles, 80 to 100 µs as the clock allows (2.1 to 1.7 GHz under it):
+// 690 to 850 TFLOP/s (a large library product: 1157). 33 rounds of two tiles take 3870
+// cycles each, in which a SIMD's two waves hold the matrix unit for 2048 and the vector
+// unit for about as long, and the LDS works for a quarter; leaving out the loads, the
+// exponentials, the sums or a product's three quarters saves 9 µs, 5, 3 or 13 each. The
+// two waves pass the same barrier and want the same unit at a time, so a round is
+// nearly the sum of both. (The teams half a round apart, by a second barrier: 3 µs
+// more.) Beside its rounds a workgroup takes 17000 cycles: 4300 to its first loads, 5800
+// for its first tile and q to arrive, 5200 to join its teams and store.
 //
 // 16-bit products take the weights rounded to the type; a row's sum is of the same
 // rounded weights, two a dot product, so that their errors cancel where few weights
@@ -268,7 +270,6 @@ __global__ __launch_bounds__((Tile<DT, HD>::THREADS)) void prompt_kernel(PagedCa
   const int p = chunk.p0 + r / G;
   const int first = A.window && p + 1 > A.window ? p + 1 - A.window : 0;
   const int wp_min = chunk.p0 + r_a / G, wp_max = chunk.p0 + min(r_a + 31, row_b) / G;
-  const int wfirst_min = A.window && wp_min + 1 > A.window ? wp_min + 1 - A.window : 0;
   const int wfirst_max = A.window && wp_max + 1 > A.window ? wp_max + 1 - A.window : 0;
 
   uint4 qf[T::QS];
