@@ -30,7 +30,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     bfloat16 or float16): log probabilities, entropies and the `top` (up to 64)
     most likely tokens. Logits of -inf have probability 0. A token outside
     [0, vocab) scores NaN, as does every value of a row that holds a NaN, a +inf
-    or nothing above -inf. Runs on torch's current stream; nothing synchronises.
+    or nothing above -inf. There is no gradient: logits that require one give plain
+    values. The four outputs share one allocation, which any of them keeps. Runs
+    on torch's current stream; nothing synchronises.
     """
     out = _lib.tensorcall().logprobs(logits, tokens, top)
     if out is not None:

@@ -18,7 +18,9 @@ positions (a power of two); any number of query heads per key/value head. Every
 call runs on torch's current stream, reads lengths, positions and page numbers
 on the device (none synchronises) and may be captured into a HIP graph. Page
 numbers outside the pool are treated as no page. There is no CPU path and no
-gradient.
+gradient (inputs that require one give plain outputs). What free_pages,
+fork_pages and compact_pages return shares one allocation a call, their
+workspace in it: an output that is kept keeps all of it.
 
 Each function first hands its call to the compiled path (csrc_py/tensorcall.cpp),
 which takes arguments that are as the kernels want them; what it leaves is

@@ -13,8 +13,10 @@ end and be packed together, and scores tokens:
 
 The reference's generation recomputes the prefix each step
 (ssalaad/inference/generate.py:1-26) and keeps no cache. Pages are given out on
-the host's count of each sequence's length; only a step that needs a new page
-waits for the device (for the free pages' numbers).
+the host's count of each sequence's length. A step copies its sequences,
+positions and lengths from host memory and so waits for the device's earlier
+work; one that needs a new page also reads the free ones' numbers, and a fork
+whether it was served.
 """
 
 from __future__ import annotations
