@@ -2,6 +2,8 @@
 // it and the host's checks of the caller's description.
 #pragma once
 
+#include <atomic>
+
 #include "abi_internal.h"
 #include "slr_common.h"
 
@@ -139,6 +141,10 @@ __device__ __forceinline__ float rounded(float x) {
 // product minus the rounded maximum is off by at most 2^-4 in the exponent, for all
 // of a row alike; above, a half step of the maximum would overflow the weights.)
 constexpr float kFarScore = 1048576.f;
+
+// Lets `kernel` take `bytes` of dynamic shared memory on the current device; `raised`
+// holds a bit a device on which it may, and starts at 0.
+int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>* raised);
 
 // Few rows of a key/value head (paged_decode.hip), or many (paged_prompt.hip).
 // The plans fill the split and return the bytes of the parts.

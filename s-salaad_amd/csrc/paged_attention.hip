@@ -18,6 +18,20 @@
 using namespace ssl;
 
 namespace ssl {
+
+int allow_lds(const void* kernel, int bytes, std::atomic<uint64_t>* raised) {
+  int dev = 0;
+  if (int rc = check_hip(hipGetDevice(&dev), "device query")) return rc;
+  const uint64_t bit = dev >= 0 && dev < 64 ? 1ull << dev : 0;
+  if (raised->load(std::memory_order_relaxed) & bit) return SSL_OK;
+  if (int rc = check_hip(
+          hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
+          "shared memory size"))
+    return rc;
+  raised->fetch_or(bit, std::memory_order_relaxed);
+  return SSL_OK;
+}
+
 namespace {
 
 // Rows of one key/value head the kernel for few of them is considered for, which

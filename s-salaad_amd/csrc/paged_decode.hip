@@ -357,18 +357,10 @@ int launch_waves(const PagedCache& C, const AttnArgs& A, int64_t max_tokens, hip
   const int n_blocks = (int)std::max<int64_t>(1, (max_tokens * G + kRows - 1) / kRows);
   const size_t lds = NW * sizeof(float) * HD * std::min<int64_t>(max_rows(A, G), kRows);
   if (lds + 4096 > 64 * 1024) {  // beside the static arrays
-    static bool raised[64] = {};  // per device
-    int dev = 0;
-    if (int rc = check_hip(hipGetDevice(&dev), "device query")) return rc;
-    if (dev < 0 || dev >= 64 || !raised[dev]) {
-      if (int rc = check_hip(
-              hipFuncSetAttribute((const void*)decode_kernel<DT, HD, NW, CHUNKS>,
-                                  hipFuncAttributeMaxDynamicSharedMemorySize,
-                                  NW * (int)sizeof(float) * HD * kRows),
-              "shared memory size"))
-        return rc;
-      if (dev >= 0 && dev < 64) raised[dev] = true;
-    }
+    static std::atomic<uint64_t> raised{0};
+    if (int rc = allow_lds((const void*)decode_kernel<DT, HD, NW, CHUNKS>,
+                           NW * (int)sizeof(float) * HD * kRows, &raised))
+      return rc;
   }
   const dim3 grid((unsigned)A.n_split, (unsigned)(C.kv_heads * n_blocks),
                   (unsigned)(C.seqs + (A.cu ? 1 : 0)));

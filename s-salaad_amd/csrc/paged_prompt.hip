@@ -713,17 +713,8 @@ int launch(const PagedCache& C, const AttnArgs& A, hipStream_t st) {
   if (grid > 0x7fffffff)
     return fail(SSL_ERR_UNSUPPORTED, "paged_attention: a grid of %lld workgroups", (long long)grid);
   if (T::LDS > 64 * 1024) {
-    static bool raised[64] = {};  // per device
-    int dev = 0;
-    if (int rc = check_hip(hipGetDevice(&dev), "device query")) return rc;
-    if (dev < 0 || dev >= 64 || !raised[dev]) {
-      if (int rc = check_hip(
-              hipFuncSetAttribute((const void*)prompt_kernel<DT, HD>,
-                                  hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS),
-              "shared memory size"))
-        return rc;
-      if (dev >= 0 && dev < 64) raised[dev] = true;
-    }
+    static std::atomic<uint64_t> raised{0};
+    if (int rc = allow_lds((const void*)prompt_kernel<DT, HD>, T::LDS, &raised)) return rc;
   }
   hipLaunchKernelGGL((prompt_kernel<DT, HD>), dim3((unsigned)grid), dim3(T::THREADS), T::LDS, st, C,
                      A, n_tiles);

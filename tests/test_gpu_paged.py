@@ -909,6 +909,42 @@ def test_a_captured_step_replays(gpu_device):
         q.add_(0)  # eager work between the replays
 
 
+def test_calls_of_several_threads(gpu_device):
+    """Eight threads, a stream each, whose first calls of these kernels meet."""
+    import threading
+
+    import ssalaad_amd as sa
+
+    dev, g = gpu_device, torch.Generator().manual_seed(15)
+    table, pages = pc.pages_of([300], 16, g)
+    td, L = table.to(dev), torch.tensor([300], dtype=torch.int32, device=dev)
+    cu = torch.tensor([0, 90], dtype=torch.int32, device=dev)
+    kinds = [(DT[dt], hd) for dt in ("f32", "bf16", "f16") for hd in (128, 256)]
+    data = {k: tuple(t.to(dev) for t in (*pc.cache(pages, 1, 16, k[1], k[0], g),
+                                         torch.randn(90, 8, k[1], generator=g).to(k[0])))
+            for k in kinds}
+    torch.cuda.synchronize()
+    results, start = [None] * 8, threading.Barrier(8)
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream(dev)):
+            start.wait()
+            results[i] = [f for kp, vp, q in data.values()
+                          for f in (sa.paged_prompt_attention(q, kp, vp, td, L, cu),
+                                    sa.paged_decode_attention(q[:1], kp, vp, td, L))]
+            torch.cuda.current_stream(dev).synchronize()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(8)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for r in results[1:]:
+        for a, b in zip(r, results[0], strict=True):
+            assert torch.equal(a, b)
+    assert all(bool(a.isfinite().all()) and bool(a.any()) for a in results[0])
+
+
 # ------------------------------------------------------------- call paths --
 class _Nothing:
     """A compiled path that takes no call."""
