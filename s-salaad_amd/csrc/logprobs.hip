@@ -136,22 +136,7 @@ struct Row {
   __device__ __forceinline__ uint4 raw(int v) const {
     return *(const uint4*)(x + peel * Elem<DT>::bytes + (int64_t)v * 16);
   }
-  __device__ __forceinline__ void vec(float* f, int v) const { unpack(f, raw(v)); }
-  __device__ __forceinline__ static void unpack(float* f, const uint4 r) {
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == DT_F32) {
-        f[i] = __uint_as_float(w[i]);
-      } else if constexpr (DT == DT_BF16) {
-        f[2 * i] = bf16_to_f32(w[i] & 0xffffu);
-        f[2 * i + 1] = bf16_to_f32(w[i] >> 16);
-      } else {
-        f[2 * i] = f16_to_f32(w[i] & 0xffffu);
-        f[2 * i + 1] = f16_to_f32(w[i] >> 16);
-      }
-    }
-  }
+  __device__ __forceinline__ void vec(float* f, int v) const { unpack16<DT>(f, raw(v)); }
   __device__ __forceinline__ float at(int i) const { return load_scalar<DT>(x, i); }
 };
 
@@ -243,7 +228,7 @@ __global__ __launch_bounds__(NT) void logprobs_kernel(LogprobArgs A) {
   while (v < R.vecs) {
     float x[U * VE];
 #pragma unroll
-    for (int u = 0; u < U; ++u) R.unpack(x + u * VE, ahead[u]);
+    for (int u = 0; u < U; ++u) unpack16<DT>(x + u * VE, ahead[u]);
     const int last = v + (U - 1) * NT;
     if (v + U * NT < R.vecs) load(v + U * NT);
     if (last >= R.vecs) {

@@ -68,20 +68,7 @@ template <int DT>
 struct Vec {
   static constexpr int VE = 16 / Elem<DT>::bytes;  // elements of a 16-byte vector
   __device__ __forceinline__ static void load(float* f, const void* base, int64_t off) {
-    const uint4 r = *(const uint4*)((const char*)base + off * Elem<DT>::bytes);
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if constexpr (DT == DT_F32) {
-        f[i] = __uint_as_float(w[i]);
-      } else if constexpr (DT == DT_BF16) {
-        f[2 * i] = bf16_to_f32(w[i] & 0xffffu);
-        f[2 * i + 1] = bf16_to_f32(w[i] >> 16);
-      } else {
-        f[2 * i] = f16_to_f32(w[i] & 0xffffu);
-        f[2 * i + 1] = f16_to_f32(w[i] >> 16);
-      }
-    }
+    unpack16<DT>(f, *(const uint4*)((const char*)base + off * Elem<DT>::bytes));
   }
   __device__ __forceinline__ static void store(void* base, int64_t off, const float* f) {
     uint32_t w[4];

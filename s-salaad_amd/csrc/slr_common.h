@@ -134,6 +134,24 @@ __device__ __forceinline__ float load_scalar(const void* p, int64_t i) {
   else if constexpr (DT == DT_BF16) return bf16_to_f32(((const uint16_t*)p)[i]);
   else return f16_to_f32(((const uint16_t*)p)[i]);
 }
+
+// The elements of 16 bytes.
+template <int DT>
+__device__ __forceinline__ void unpack16(float* f, const uint4 r) {
+  const uint32_t w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == DT_F32) {
+      f[i] = __uint_as_float(w[i]);
+    } else if constexpr (DT == DT_BF16) {
+      f[2 * i] = bf16_to_f32(w[i] & 0xffffu);
+      f[2 * i + 1] = bf16_to_f32(w[i] >> 16);
+    } else {
+      f[2 * i] = f16_to_f32(w[i] & 0xffffu);
+      f[2 * i + 1] = f16_to_f32(w[i] >> 16);
+    }
+  }
+}
 template <int DT>
 __device__ __forceinline__ uint32_t to_bits(float f) {
   if constexpr (DT == DT_BF16) return f32_to_bf16(f);
