@@ -282,3 +282,29 @@ def test_logits_in_16_bits(model_type, hd, dtype, gpu_device):
     eng.fork([0], [2])
     got = eng.feed([2, 0], [text[66:], text[66:70]], all_logits=True)
     assert _err(got, torch.cat([want[66:], want[66:70]])) <= tol
+
+
+@pytest.mark.parametrize("model_type,kv", [("llama", 4), ("llama", 2), ("qwen3", 2)])
+@pytest.mark.parametrize("dtype,nm", [(torch.float32, False), (torch.bfloat16, False),
+                                      (torch.bfloat16, True)])
+def test_a_compressed_model_is_served(model_type, kv, dtype, nm, gpu_device):
+    """SLR projections: a prompt, steps of two sequences, a fork and a further chunk,
+    against the dense twin in float64. fp32: the decode engine's bar; bf16: twice the
+    error of the reference module's own arithmetic, or 3e-2. (2:4 S is 16-bit.)"""
+    from ssalaad_amd import PagedEngine
+    from test_gpu_decode import _slr_triple
+
+    model, dense, mirror = _slr_triple(model_type, dtype, kv, gpu_device, seed=5, nm=nm)
+    eng = PagedEngine(model.to(gpu_device).eval(), max_seqs=3, pages=30, page=16)
+    g = torch.Generator().manual_seed(6)
+    text = torch.randint(0, 384, (100,), generator=g)
+    with torch.no_grad():
+        want = dense.eval()(text[None]).logits[0]
+        tol = TOL if dtype == torch.float32 else min(
+            3e-2, 2 * _err(mirror(text[None]).logits[0], want))
+    got = [eng.feed([0], [text[:70]], all_logits=True)]
+    for t in range(70, 80):
+        got.append(eng.step([0], text[t: t + 1]))
+    eng.fork([0], [2])
+    got.append(eng.feed([2, 0], [text[80:], text[80:85]], all_logits=True))
+    assert _err(torch.cat(got), torch.cat([want, want[80:85]])) <= tol
