@@ -214,30 +214,31 @@ class PagedEngine:
                 rows: torch.Tensor | None = None) -> torch.Tensor:
         """Append new tokens, counts[i] of seqs[i]: their logits, or those of `rows`
         of them. The sequences grow when all has been issued."""
-        x = self._forward(tokens, seqs, counts)
-        logits = self.lm_head(x if rows is None else x[rows])
+        at = self._ints(seqs).long()
         ends = [self._host_lengths[s] + n for s, n in zip(seqs, counts)]
-        self.lengths[self._ints(seqs).long()] = self._ints(ends)
+        lengths = self._ints(ends)
+        x = self._forward(tokens, seqs, counts, at, lengths, max(ends))
+        logits = self.lm_head(x if rows is None else x[rows])
+        self.lengths[at] = lengths
         for s, n in zip(seqs, ends):
             self._host_lengths[s] = n
         return logits
 
-    def _forward(self, tokens: torch.Tensor, seqs: list[int], counts: list[int]) -> torch.Tensor:
-        """The final hidden states of new tokens, counts[i] of seqs[i]."""
+    def _forward(self, tokens: torch.Tensor, seqs: list[int], counts: list[int],
+                 at: torch.Tensor, lengths: torch.Tensor, longest: int) -> torch.Tensor:
+        """The final hidden states of new tokens, counts[i] of seqs[i] (`at` on the
+        device), which come to `lengths` by them."""
         starts = [self._host_lengths[s] for s in seqs]
-        ends = [a + n for a, n in zip(starts, counts)]
         self._reserve(seqs, counts)
         owners = self._ints([s for s, n in zip(seqs, counts) for _ in range(n)])
         positions = self._ints([a + j for a, n in zip(starts, counts) for j in range(n)])
-        lengths = self._ints(ends)
-        table = self.table[self._ints(seqs).long()]
-        longest = max(ends)
+        table = self.table[at]
         cu = None
         if max(counts) > 1:
-            at = [0]
+            edges = [0]
             for n in counts:
-                at.append(at[-1] + n)
-            cu = self._ints(at)
+                edges.append(edges[-1] + n)
+            cu = self._ints(edges)
         n, H, KH, hd = tokens.numel(), self.heads, self.kv_heads, self.head_dim
         for i, L in enumerate(self.layers):
             if i == 0:
